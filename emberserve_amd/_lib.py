@@ -15,7 +15,7 @@ import torch
 from torch.compiler import is_dynamo_compiling as tracing  # noqa: F401  (for the callers of `fast`)
 
 LIB_PATH = Path(__file__).resolve().parent / "libember_ops.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 F32, F16, BF16 = 0, 1, 2
 ERR_EMBED_ID = 1
@@ -109,6 +109,17 @@ SIGNATURES: dict[str, list] = {
     "ember_moe_align_padded_size": [_i64, _i64, _i64],
     "ember_moe_align_workspace_bytes": [_i64, _i64],
     "ember_moe_align": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+    "ember_w4_packed_bytes": [_i64, _i64, _i64, _i32],
+    "ember_w4_pack_weight": [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p,
+                             _p],
+    "ember_w4_linear": [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _i64, _p],
+    "ember_w4_gate_up_silu": [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p],
+    "ember_moe_layer_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ember_moe_layer": [_p, _i64, _p, _i32, _p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64,
+                        _i64, _p, _i64, _p, _i64, _p],
+    "ember_moe_layer_w4": [_p, _i64, _p, _i32, _p, _i32, _i64, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p,
+                           _i64, _p, _i64, _p],
+    "ember_moe_down_pack_weight": [_p, _i64, _i64, _i32, _i64, _i64, _i64, _p, _p],
     "ember_read_errors": [ctypes.POINTER(ctypes.c_uint32), _i32],
     "ember_stream_capture_id": [_p, ctypes.POINTER(ctypes.c_uint64)],
     "ember_abi_version": [],
@@ -119,6 +130,8 @@ _RESTYPE = {"ember_status_string": ctypes.c_char_p, "ember_paged_decode_workspac
             "ember_mla_decode_workspace_bytes": ctypes.c_int64,
             "ember_gate_up_silu_workspace_bytes": ctypes.c_int64,
             "ember_moe_gate_up_silu_workspace_bytes": ctypes.c_int64,
+            "ember_w4_packed_bytes": ctypes.c_int64,
+            "ember_moe_layer_workspace_bytes": ctypes.c_int64,
             "ember_moe_align_padded_size": ctypes.c_int64,
             "ember_moe_align_workspace_bytes": ctypes.c_int64,
             "ember_paged_decode_noalloc_max_bytes": ctypes.c_int64}

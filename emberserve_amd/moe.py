@@ -8,22 +8,26 @@ block-aligned expert layout (`moe_align`, moe_triton.py:215-254).
         -> act [N * k, I],  act[t * k + c] = silu_and_mul(x[t] @ w_gate_up[topk_ids[t, c]].T)
 
 with the linear layer's output rounded to the activation dtype before the activation, as
-`_grouped_gemm` stores it. The down projection and the routed-weight sum stay the
-caller's (moe_triton.py:341-345).
+`_grouped_gemm` stores it. At prefill sizes the down projection and the routed-weight sum stay
+the caller's (moe_triton.py:341-345); for up to 64 tokens `fused_moe` is the whole layer, in two
+launches (`ember_moe_layer`), over 16-bit or 4-bit experts.
 
 CPU tensors, or `EMBERSERVE_FUSED_OPS=0`, take an eager per-block form.
 """
 
 from __future__ import annotations
 
+from ctypes import byref, c_int64
+
 import torch
 import torch.nn.functional as F
 from torch import Tensor
 
 from . import _lib, ops
-from ._scratch import ScratchCache, round_up
+from ._scratch import ScratchCache, SharedScratch, round_up
 from .ops import _check_indices, _launch, _require_device, fused_enabled
 from .paged_decode import num_sms
+from .w4 import PackedW4
 
 BLOCK_M = 16  # assignments per block (moe_triton.py:38)
 SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
@@ -442,3 +446,164 @@ def fused_moe_gate_up(x: Tensor, topk_ids: Tensor, w_gate_up: Tensor, *, num_spl
     sorted_ids, block_expert, num_valid = moe_align(topk_ids, E)
     return moe_gate_up_silu(x, w_gate_up, sorted_ids, block_expert, num_valid, k,
                             num_splits=num_splits, packed=packed)
+
+
+# ---- the whole layer for decode batches ---------------------------------------------------
+
+LAYER_MAX_TOKENS = 64
+LAYER_MAX_ASSIGNMENTS = 512
+LAYER_MAX_EXPERTS = 1024
+
+# Activations, group lists, split partials and arrival counters of ember_moe_layer: two launches share
+# them, so one buffer per (thread, device, stream).
+_LAYER_SCRATCH = SharedScratch("fused_moe")
+
+
+class PackedDown:
+    """The routed experts' down weights [E, H, I] rearranged for `ember_moe_layer`: slabs of 16 rows,
+    each one contiguous stream of MFMA operand fragments. Made once per weight by
+    `pack_moe_down_weight`; the same bytes as the weight."""
+
+    def __init__(self, packed: Tensor, num_experts: int, hidden: int, inter: int) -> None:
+        self.packed, self.num_experts, self.hidden, self.inter = packed, num_experts, hidden, inter
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.packed.dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+
+def pack_moe_down_weight(w_down: Tensor) -> PackedDown:
+    """The packed copy of w_down [E, H, I] (fp16/bf16 on the GPU, H and I multiples of 64)."""
+    if w_down.dim() != 3 or w_down.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"pack_moe_down_weight: an [E, H, I] fp16/bf16 weight expected, got {tuple(w_down.shape)} "
+                         f"{w_down.dtype}")
+    _require_device("pack_moe_down_weight", w_down)
+    E, H, I = w_down.shape
+    if (0 in w_down.shape or H % 64 or I % 64 or w_down.stride(2) != 1 or w_down.stride(1) % 8 or w_down.stride(0) % 8
+            or w_down.data_ptr() % 16):
+        raise ValueError("pack_moe_down_weight: H and I must be multiples of 64, rows unit-stride and 16-byte aligned")
+    packed = torch.empty(E * H * I, dtype=w_down.dtype, device=w_down.device)
+    _launch("ember_moe_down_pack_weight", _lib.load().ember_moe_down_pack_weight, w_down.device, w_down.data_ptr(),
+            w_down.stride(0), w_down.stride(1), _lib.dtype_tag(w_down.dtype), E, H, I, packed.data_ptr())
+    return PackedDown(packed, E, H, I)
+
+
+def fused_moe_torch(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
+    """Eager form: every routed expert over its tokens, in fp32, rounded once."""
+    y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+    experts = w_gate_up.shape[0]
+    for e in sorted(set(topk_ids.reshape(-1).tolist())):
+        if 0 <= e < experts:
+            rows, choice = (topk_ids == e).nonzero(as_tuple=True)
+            g, u = F.linear(x[rows].float(), w_gate_up[e].float()).chunk(2, dim=-1)
+            part = F.linear(F.silu(g) * u, w_down[e].float())
+            y.index_add_(0, rows, topk_weights[rows, choice].float()[:, None] * part)
+    return y.to(x.dtype)
+
+
+def _layer_rows(w: Tensor, what: str) -> tuple[int, int, int]:
+    """An unpacked expert weight's (pointer, expert stride, row stride)."""
+    if w.stride(2) != 1 or w.stride(1) % 8 or w.stride(0) % 8 or w.stride(1) < w.shape[2] or w.data_ptr() % 16:
+        raise ValueError(f"fused_moe: {what} needs unit inner stride, rows a multiple of 8 elements apart and 16-byte "
+                         "alignment")
+    return w.data_ptr(), w.stride(0), w.stride(1)
+
+
+def _layer_weight(what: str, w: Tensor | None, packed, gate_up: bool):
+    """(the weight that the layer reads, (E, H, I), dtype or None for 4 bits, device)."""
+    if packed is not None:
+        if isinstance(packed, PackedW4):
+            if packed.gate_up != gate_up or packed.num_experts is None:
+                raise ValueError(f"fused_moe: {what} is {packed}, experts from "
+                                 f"{'pack_w4_gate_up' if gate_up else 'pack_w4'} expected")
+            h, i = (packed.k, packed.rows) if gate_up else (packed.rows, packed.k)
+            return packed, (packed.num_experts, h, i), None, packed.device
+        if not isinstance(packed, PackedExperts if gate_up else PackedDown):
+            raise TypeError(f"fused_moe: {what} cannot be a {type(packed).__name__}")
+        return packed, (packed.num_experts, packed.hidden, packed.inter), packed.dtype, packed.device
+    if w is None:
+        raise ValueError(f"fused_moe: {'w_gate_up' if gate_up else 'w_down'} or {what} is needed")
+    if w.dim() != 3 or (gate_up and w.shape[1] % 2):
+        raise ValueError(f"fused_moe: {'w_gate_up [E, 2I, H]' if gate_up else 'w_down [E, H, I]'} expected, got "
+                         f"{tuple(w.shape)}")
+    e, n, k = w.shape
+    return w, ((e, k, n // 2) if gate_up else (e, n, k)), w.dtype, w.device
+
+
+def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor | None, w_down: Tensor | None, *,
+              packed: PackedExperts | PackedW4 | None = None, packed_down: PackedDown | PackedW4 | None = None) -> Tensor:
+    """The routed experts' layer of fused_moe_forward (moe_triton.py:332-345) for a decode step:
+
+        out[t] = round(sum_c topk_weights[t, c] * silu_and_mul(x[t] @ w_gate_up[e].T) @ w_down[e].T),  e = topk_ids[t, c]
+
+    x [N, H] fp16/bf16 with N <= LAYER_MAX_TOKENS and N k <= LAYER_MAX_ASSIGNMENTS, topk_ids [N, k]
+    int32/int64, topk_weights [N, k] fp32/fp16/bf16, w_gate_up [E, 2I, H], w_down [E, H, I]. `packed`
+    (`pack_moe_gate_up_weight`, the copy `fused_moe_gate_up` also reads) and `packed_down`
+    (`pack_moe_down_weight`) are read instead where given, and the weight may then be None; both may
+    be 4-bit (`w4.pack_w4_gate_up` and `w4.pack_w4` of [E, ...] codes). The activations are rounded
+    once, to x's dtype, between the products; the sums are fp32. An id of -1 adds nothing; other ids
+    outside [0, E) neither, and set the error word. H and I are multiples of 64 (4-bit: of 32 and of
+    their groups)."""
+    for name, t in (("x", x), ("topk_ids", topk_ids), ("topk_weights", topk_weights)):
+        if t.dim() != 2:
+            raise ValueError(f"fused_moe: {name} must have two dimensions, got {tuple(t.shape)}")
+    w1, (E, H, I), dt1, dev1 = _layer_weight("packed", w_gate_up, packed, True)
+    w2, shape2, dt2, dev2 = _layer_weight("packed_down", w_down, packed_down, False)
+    n, k = topk_ids.shape
+    if x.shape != (n, H) or topk_weights.shape != (n, k) or shape2 != (E, H, I):
+        raise ValueError(f"fused_moe: x {tuple(x.shape)}, topk_ids {tuple(topk_ids.shape)}, topk_weights "
+                         f"{tuple(topk_weights.shape)}, gate_up {(E, H, I)} and down {shape2} (E, H, I) do not match")
+    if x.dtype not in SUPPORTED_DTYPES or dt1 not in (None, x.dtype) or dt2 not in (None, x.dtype):
+        raise TypeError(f"fused_moe: fp16 or bf16 x and weights of its dtype expected, got {x.dtype}, {dt1}, {dt2}")
+    if (dt1 is None) != (dt2 is None):
+        raise ValueError("fused_moe: gate_up and down must both be 4-bit or both 16-bit")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"fused_moe: int32/int64 topk_ids expected, got {topk_ids.dtype}")
+    if topk_weights.dtype not in (torch.float32, *SUPPORTED_DTYPES):
+        raise TypeError(f"fused_moe: fp32, fp16 or bf16 topk_weights expected, got {topk_weights.dtype}")
+    for t in (topk_ids.device, topk_weights.device, dev1, dev2):
+        if t != x.device:
+            raise ValueError(f"fused_moe: all tensors must be on {x.device}, got one on {t}")
+    if k < 1 or n > LAYER_MAX_TOKENS or n * k > LAYER_MAX_ASSIGNMENTS or E > LAYER_MAX_EXPERTS:
+        raise ValueError(f"fused_moe: up to {LAYER_MAX_TOKENS} tokens, {LAYER_MAX_ASSIGNMENTS} assignments and "
+                         f"{LAYER_MAX_EXPERTS} experts, got {n} x {k} over {E} (fused_moe_gate_up takes more)")
+    w4 = dt1 is None
+    if not fused_enabled(x):
+        a, b = (w.dequantize(torch.float32) for w in (w1, w2)) if w4 else (w_gate_up, w_down)
+        if a is None or b is None:
+            raise ValueError("fused_moe: the eager form needs the unpacked weights")
+        return fused_moe_torch(x, topk_ids, topk_weights, a, b)
+    if not w4 and (H % 64 or I % 64):
+        raise ValueError(f"fused_moe: H and I must be multiples of 64, got {H} and {I}")
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
+    out = torch.empty((n, H), dtype=x.dtype, device=x.device)
+    if n == 0:
+        return out
+    lib = _lib.load()
+    counters = c_int64(0)
+    need = lib.ember_moe_layer_workspace_bytes(n, k, E, H, I, byref(counters))
+    if need < 0:
+        raise ValueError(f"fused_moe: H {H} and I {I} not supported")
+    ws = _LAYER_SCRATCH.get(need - counters.value, counters.value, x.device)
+    head = (x.data_ptr(), x.stride(0), ids.data_ptr(), ids.element_size(), weights.data_ptr(),
+            _lib.dtype_tag(weights.dtype), n, k)
+    tail = (_lib.dtype_tag(x.dtype), E, H, I, ws.data_ptr(), ws.numel() * 4, out.data_ptr(), out.stride(0))
+    if w4:
+        _launch("ember_moe_layer_w4", lib.ember_moe_layer_w4, x.device, *head, w1.packed.data_ptr(), w1.group,
+                w2.packed.data_ptr(), w2.group, *tail)
+    else:
+        up = _layer_rows(w1, "w_gate_up") if packed is None else (w1.packed.data_ptr(), 0, 0)
+        down = _layer_rows(w2, "w_down") if packed_down is None else (w2.packed.data_ptr(), 0, 0)
+        _launch("ember_moe_layer", lib.ember_moe_layer, x.device, *head, *up, *down, *tail)
+    if _check_indices():
+        end = ws.numel() * 4
+        _LAYER_SCRATCH.verify_counters(ws, end - counters.value, end)
+        if _lib.read_errors(clear=True) & _lib.ERR_EXPERT_ID:
+            raise IndexError(f"emberserve_amd.fused_moe: expert id outside [0, {E})")
+    return out

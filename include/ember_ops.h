@@ -60,6 +60,11 @@
  *                             (also _packed, _direct for decode batches, _gemm at prefill)
  *   ember_moe_align           moe_align, emberserve/model/moe_triton.py:215-254 (one
  *                             workgroup, or a count + place grid with a workspace)
+ *   ember_moe_layer           fused_moe_forward, emberserve/model/moe_triton.py:332-345, for decode
+ *                             batches (also _w4: over 4-bit experts)
+ *   ember_w4_linear           no counterpart: projections over 4-bit weights with group scales (the
+ *                             reference's weight-only path is int8, emberserve/model/quant.py:113)
+ *   ember_w4_gate_up_silu     no counterpart: ember_gate_up_silu over such a weight
  *   ember_mla_decode          mla_decode, emberserve/attn/mla_triton.py:119-182 (kernel
  *                             :49-116; fp32 definition attn/mla_torch.py:33-53)
  *   ember_mla_decode_workspace_bytes  its split-K scratch size (the _SCRATCH buffers,
@@ -610,6 +615,82 @@ int64_t ember_moe_align_workspace_bytes(int64_t num_valid, int64_t num_experts);
 int ember_moe_align(const void* topk_ids, int id_bytes, int64_t num_valid, int64_t num_experts, int64_t block_m,
                     int32_t* sorted_ids, int64_t max_padded, int32_t* block_expert, int64_t max_blocks,
                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- 4-bit weights with group scales ----
+ * A weight [rows, k] held as codes q in 0..15, scales s and zero points z in 0..15, one of each per
+ * (row, group of k): w[n, j] = s[n, j / group] * (q[n, j] - z[n, j / group]). group is 32, 64 or a
+ * multiple of 128, and divides k. */
+
+/* Bytes of one expert's (or the only) packed weight, -1 for invalid arguments: slabs of 16 rows,
+ * each ceil(k / 128) blocks of 1024 + 64 gpb bytes, gpb = 128 / group groups a block (1 from 128
+ * on). gate_up: rows is one half's; gate and up slabs alternate. */
+int64_t ember_w4_packed_bytes(int64_t rows, int64_t k, int64_t group, int gate_up);
+
+/* Packs codes [num_experts, rows, k / 2] (two to a byte, the even k in the low nibble), scales
+ * [num_experts, rows, k / group] (scale_dtype EMBER_F16 or EMBER_BF16) and zeros (uint8, like the
+ * scales; NULL: 8 everywhere) for the entry points below, once per weight. With gate_up the inputs
+ * have 2 rows rows, gate then up. Strides are in elements (bytes for the codes). packed holds
+ * num_experts * ember_w4_packed_bytes bytes, 16-byte aligned:
+ *   block[lane][f]: the codes of row lane % 16 of the slab at k = 128 b + 32 f + 8 (lane / 16) + j,
+ *                   j < 8, at bits 4 (j / 2) + 16 (j % 2)                (lane < 64, f < 4)
+ *   then [row][gpb] words: the scale as fp32 bits, with its zero point in the low four bits. */
+int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t code_row_stride, const void* scales,
+                         int64_t scale_expert_stride, int64_t scale_row_stride, int scale_dtype, const void* zeros,
+                         int64_t zero_expert_stride, int64_t zero_row_stride, int64_t num_experts, int64_t rows,
+                         int64_t k, int64_t group, int gate_up, void* packed, void* stream);
+
+/* out[t, n] = round(x[t] . w[n] + bias[n]) over a packed 4-bit weight, x [tokens, k] and out
+ * [tokens, rows] fp16 or bf16 (dtype), bias [rows] of that dtype or NULL. Unit inner strides; x 16-byte
+ * aligned with a row stride that is a multiple of 8 (EMBER_EALIGN otherwise). Sums are fp32, rounded
+ * once. Any number of tokens up to 2^21; 64 of them share a pass over the weight. */
+int ember_w4_linear(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype, int64_t tokens,
+                    int64_t k, int64_t rows, const void* bias, void* out, int64_t out_row_stride, void* stream);
+
+/* out[t, j] = round(silu(g) * u), g and u the fp32 products of x[t] with gate row j and up row j of a
+ * weight packed with gate_up (rows = inter). Not rounded in between, unlike ember_gate_up_silu. */
+int ember_w4_gate_up_silu(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype,
+                          int64_t tokens, int64_t hidden, int64_t inter, void* out, int64_t out_row_stride,
+                          void* stream);
+
+/* ---- the routed experts' whole layer ----
+ *   act[t, c, j] = round(silu(x[t] . W1[e, j]) * (x[t] . W1[e, inter + j])),   e = topk_ids[t, c]
+ *   out[t, n]    = round(sum over c of topk_weights[t, c] * (W2[e, n] . act[t, c]))
+ * for up to 64 tokens and 512 assignments (num_tokens * top_k). Replaces fused_moe_forward,
+ * moe_triton.py:332-345, at decode sizes, in two launches with no alignment step. x and out
+ * [num_tokens, hidden] fp16 or bf16 (dtype); topk_ids [num_tokens, top_k] contiguous, int32 or int64
+ * (id_bytes); topk_weights like them, of weight_dtype. An id of -1 adds nothing (an expert of another
+ * rank); any other outside [0, num_experts) neither, and sets EMBER_ERR_EXPERT_ID. A token without
+ * experts gets zeros. w_gate_up [num_experts, 2 inter, hidden] (gate rows, then up rows) and w_down
+ * [num_experts, hidden, inter], of dtype, by strides; a row stride of 0 marks the packed forms of
+ * ember_moe_gate_up_silu_pack_weight and ember_moe_down_pack_weight. hidden and inter multiples of
+ * 64, num_experts <= 1024; x and weights 16-byte aligned, strides multiples of 8 (EMBER_EALIGN).
+ * The workspace (ember_moe_layer_workspace_bytes; more is fine, the size a multiple of 16) holds
+ * counters at its end, *counter_bytes of them, which must be zero before its first use and are left
+ * zero; calls of different shapes may take turns on one workspace as long as no call's other part
+ * reaches another's counters. Calls that overlap on one workspace race. */
+int64_t ember_moe_layer_workspace_bytes(int64_t num_tokens, int64_t top_k, int64_t num_experts, int64_t hidden,
+                                        int64_t inter, int64_t* counter_bytes);
+int ember_moe_layer(const void* x, int64_t x_row_stride, const void* topk_ids, int id_bytes, const void* topk_weights,
+                    int weight_dtype, int64_t num_tokens, int64_t top_k, const void* w_gate_up,
+                    int64_t gate_up_expert_stride, int64_t gate_up_row_stride, const void* w_down,
+                    int64_t down_expert_stride, int64_t down_row_stride, int dtype, int64_t num_experts, int64_t hidden,
+                    int64_t inter, void* workspace, int64_t workspace_bytes, void* out, int64_t out_row_stride,
+                    void* stream);
+
+/* ember_moe_layer over experts packed by ember_w4_pack_weight: the gate_up weight with gate_up, rows =
+ * inter, k = hidden; the down weight with rows = hidden, k = inter. hidden and inter multiples of 32
+ * that their groups divide. */
+int ember_moe_layer_w4(const void* x, int64_t x_row_stride, const void* topk_ids, int id_bytes,
+                       const void* topk_weights, int weight_dtype, int64_t num_tokens, int64_t top_k,
+                       const void* packed_gate_up, int64_t gate_up_group, const void* packed_down, int64_t down_group,
+                       int dtype, int64_t num_experts, int64_t hidden, int64_t inter, void* workspace,
+                       int64_t workspace_bytes, void* out, int64_t out_row_stride, void* stream);
+
+/* Rearranges w_down [num_experts, hidden, inter] (element strides, fp16 or bf16, 16-byte aligned; hidden
+ * a multiple of 16, inter of 64) for ember_moe_layer: packed[e][n / 16][j / 32][lane][8] =
+ * w[e][16 (n / 16) + lane % 16][32 (j / 32) + 8 (lane / 16) + 0..7]. A pure permutation. */
+int ember_moe_down_pack_weight(const void* w, int64_t w_expert_stride, int64_t w_row_stride, int dtype,
+                               int64_t num_experts, int64_t hidden, int64_t inter, void* packed, void* stream);
 
 #ifdef __cplusplus
 }

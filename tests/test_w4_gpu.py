@@ -1,0 +1,182 @@
+"""4-bit projections (`w4.linear_w4`, `w4.gate_up_silu_w4`) on the GPU against 64-bit values, with the
+bounds of tests.w4_bounds."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+from emberserve_amd import _lib, w4  # noqa: E402
+from tests.w4_bounds import act_bound, check, codes64, dot_bound  # noqa: E402
+
+DEV = "cuda"
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _weight(n, k, group, zeros, dtype, seed, experts=None):
+    g = torch.Generator().manual_seed(seed)
+    lead = () if experts is None else (experts,)
+    q = torch.randint(0, 256, (*lead, n, k // 2), generator=g, dtype=torch.uint8)
+    s = (torch.rand((*lead, n, k // group), generator=g) * 0.02 + 0.001).to(dtype)
+    z = torch.randint(0, 16, s.shape, generator=g, dtype=torch.uint8) if zeros else None
+    return q, s, z
+
+
+def _x(t, k, dtype, seed):
+    return torch.randn(t, k, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _dev(parts):
+    return [None if p is None else p.to(DEV) for p in parts]
+
+
+@pytest.mark.parametrize("gate_up", [False, True])
+@pytest.mark.parametrize("n,k,group", [(16, 32, 32), (20, 128, 64), (6, 192, 64), (34, 416, 32), (48, 1024, 256)])
+def test_pack_round_trip(n, k, group, gate_up):
+    parts = _weight(n, k, group, True, HF, seed=n)
+    packed = (w4.pack_w4_gate_up if gate_up else w4.pack_w4)(*_dev(parts))
+    want = w4.dequantize_w4(*parts, dtype=torch.float32)
+    assert torch.equal(packed.dequantize(torch.float32).cpu(), want)
+    stacked = [torch.stack([p, p.flip(0)]) for p in parts]
+    packed = (w4.pack_w4_gate_up if gate_up else w4.pack_w4)(*_dev(stacked))
+    assert torch.equal(packed.dequantize(torch.float32).cpu(), w4.dequantize_w4(*stacked, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,n,k,group,zeros", [
+    (1, 16, 32, 32, False), (1, 1, 64, 64, True), (3, 17, 96, 32, True), (16, 48, 896, 128, False),
+    (17, 1152, 896, 64, True), (33, 100, 4864, 128, True), (64, 272, 1024, 32, False), (65, 33, 160, 32, True),
+    (200, 64, 384, 128, False), (2, 3584, 2048, 512, True), (5, 40000, 256, 128, False), (31, 70001, 128, 64, True),
+    (50, 70000, 64, 32, False)])
+def test_linear_matches_64_bits(dtype, t, n, k, group, zeros):
+    print(f"linear_w4 {t}x{n}x{k} g{group} zeros={zeros} {dtype}", flush=True)
+    parts, x = _weight(n, k, group, zeros, dtype, seed=t + n), _x(t, k, dtype, seed=k)
+    w, s = codes64(*parts)
+    want, bound = dot_bound(x, w, s, group)
+    packed = w4.pack_w4(*_dev(parts))
+    got = w4.linear_w4(x.to(DEV), packed)
+    assert got.dtype == dtype and got.shape == (t, n)
+    check(got, want, bound, "no bias")
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(1)).to(dtype)
+    got = w4.linear_w4(x.to(DEV), packed, bias.to(DEV))
+    check(got, want + bias.double(), bound + 2.0 ** -23 * (want.abs() + bias.double().abs()), "bias")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,inter,k,group,zeros", [
+    (1, 16, 32, 32, True), (2, 5, 128, 128, False), (16, 4864, 896, 128, True), (27, 77, 416, 32, True),
+    (64, 160, 512, 64, False), (70, 30, 256, 256, True), (9, 40000, 128, 64, False), (40, 33000, 64, 32, True)])
+def test_gate_up_matches_64_bits(dtype, t, inter, k, group, zeros):
+    print(f"gate_up_silu_w4 {t}x{inter}x{k} g{group} zeros={zeros} {dtype}", flush=True)
+    parts, x = _weight(2 * inter, k, group, zeros, dtype, seed=t + inter), _x(t, k, dtype, seed=k)
+    w, s = codes64(*parts)
+    want, bound = act_bound(*dot_bound(x, w, s, group))
+    got = w4.gate_up_silu_w4(x.to(DEV), w4.pack_w4_gate_up(*_dev(parts)))
+    check(got, want, bound)
+
+
+def test_x_strides_and_alignment():
+    """Rows far apart, rows of a transposed tensor, an odd first element: the same bits as contiguous."""
+    parts = _weight(50, 256, 64, True, BF, seed=3)
+    packed = w4.pack_w4(*_dev(parts))
+    x = _x(9, 256, BF, seed=4).to(DEV)
+    want = w4.linear_w4(x, packed)
+    wide = torch.full((9, 1024), float("nan"), dtype=BF, device=DEV)
+    wide[:, 256:512] = x
+    assert torch.equal(w4.linear_w4(wide[:, 256:512], packed), want)
+    assert torch.equal(w4.linear_w4(x.T.contiguous().T, packed), want)
+    odd = torch.zeros(9 * 256 + 1, dtype=BF, device=DEV)[1:].view(9, 256)
+    odd.copy_(x)
+    assert torch.equal(w4.linear_w4(odd, packed), want)
+    assert torch.equal(w4.linear_w4(x.view(3, 3, 256), packed), want.view(3, 3, 50))
+    assert w4.linear_w4(x[:0], packed).shape == (0, 50)
+
+
+def test_pack_of_strided_parts():
+    """Codes, scales and zeros as views of wider tensors pack to the same array."""
+    parts = _dev(_weight(48, 256, 64, True, HF, seed=5))
+    want = w4.pack_w4(*parts).packed
+    wide = [torch.cat([p, p.flip(0)], dim=1)[:, :p.shape[1]] for p in parts]
+    assert torch.equal(w4.pack_w4(*wide).packed, want)
+    cols = [p.T.contiguous().T for p in parts]
+    assert torch.equal(w4.pack_w4(*cols).packed, want)
+
+
+def test_nonfinite_rows_stay_their_own():
+    """A token with a NaN or an infinity gives NaN in its row and leaves the others' bits alone."""
+    parts = _weight(64, 416, 32, True, BF, seed=6)
+    packed = w4.pack_w4(*_dev(parts))
+    x = _x(20, 416, BF, seed=7).to(DEV)
+    want = w4.linear_w4(x, packed)
+    y = x.clone()
+    y[3, 415] = float("nan")
+    y[17, 0] = float("inf")
+    got = w4.linear_w4(y, packed)
+    assert bool(got[[3, 17]].isnan().all())
+    keep = [i for i in range(20) if i not in (3, 17)]
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_extreme_scales_and_values():
+    """Zero, negative and subnormal scales, and x at the largest finite value that the sum allows."""
+    q, s, z = _weight(32, 128, 32, True, HF, seed=8)
+    s[0] = 0.0
+    s[1] = -s[1]
+    s[2] = 2.0 ** -24
+    x = _x(4, 128, HF, seed=9)
+    x[1] = 60000.0
+    w, sa = codes64(q, s, z)
+    want, bound = dot_bound(x, w, sa, 32)
+    got = w4.linear_w4(x.to(DEV), w4.pack_w4(*_dev((q, s, z))))
+    small = want.abs() < 65000
+    check(torch.where(small.to(DEV), got, 0), torch.where(small, want, 0.0), bound)
+    over = want.abs() > 66000  # past fp16's range: the rounded value is infinite
+    assert bool(got.cpu()[over].isinf().all())
+
+
+def test_graph_replays_match_eager():
+    parts, gu = _weight(1152, 896, 128, False, BF, seed=10), _weight(2 * 304, 896, 128, False, BF, seed=11)
+    packed, packed_gu = w4.pack_w4(*_dev(parts)), w4.pack_w4_gate_up(*_dev(gu))
+    x = _x(3, 896, BF, seed=12).to(DEV)
+    w4.linear_w4(x, packed)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = w4.linear_w4(x, packed), w4.gate_up_silu_w4(x, packed_gu)
+    for i in range(3):
+        x.copy_(_x(3, 896, BF, seed=20 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, w4.linear_w4(x, packed)) and torch.equal(b, w4.gate_up_silu_w4(x, packed_gu)), i
+
+
+def test_another_stream():
+    parts = _weight(256, 1024, 128, False, BF, seed=13)
+    packed = w4.pack_w4(*_dev(parts))
+    x = _x(4, 1024, BF, seed=14).to(DEV)
+    want = w4.linear_w4(x, packed)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = w4.linear_w4(x, packed)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_eager_form_of_a_gpu_weight(monkeypatch):
+    """EMBERSERVE_FUSED_OPS=0 computes from the packed copy in torch."""
+    parts = _weight(40, 256, 64, True, BF, seed=15)
+    x = _x(5, 256, BF, seed=16)
+    w, s = codes64(*parts)
+    want, bound = dot_bound(x, w, s, 64)
+    packed = w4.pack_w4(*_dev(parts))
+    monkeypatch.setenv("EMBERSERVE_FUSED_OPS", "0")
+    check(w4.linear_w4(x.to(DEV), packed), want, bound + 300 * 2.0 ** -24 * (x.double().abs() @ w.abs().T))
+
+
+def test_no_error_bits():
+    assert _lib.read_errors(clear=True) == 0
