@@ -32,6 +32,24 @@ namespace ember {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+typedef __amdgpu_buffer_rsrc_t BufferRsrc;
+constexpr int kPolicyNt = 2;  // non-temporal
+
+// An offset to OR into a load's: past every resource (the load gives zeros) where `past`, else 0. Opaque,
+// or the compiler turns the choice into a branch around every load.
+__device__ __forceinline__ int nowhere(bool past) {
+  int v = past ? 0x7fffff00 : 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("" : "+v"(v));
+#endif
+  return v;
+}
+
+__device__ __forceinline__ BufferRsrc buffer(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, kBufferWord3);
+}
 
 template <typename T>
 struct Mfma16;
@@ -56,6 +74,16 @@ struct Mfma16<__bf16> {
   }
 };
 
+// (w & mask) | bias as one v_and_or_b32: gfx9 takes one scalar and no literal in it, so the mask has to sit
+// in a vector register, which the empty asm makes the compiler do; it splits two literals into two
+// instructions (12 a word of codes instead of 8).
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bias) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("" : "+v"(mask));
+#endif
+  return (w & mask) | bias;
+}
+
 // Eight codes of one word as 16 + q.
 template <typename T>
 __device__ __forceinline__ typename Mfma16<T>::v8 w4_values(uint32_t w) {
@@ -64,7 +92,7 @@ __device__ __forceinline__ typename Mfma16<T>::v8 w4_values(uint32_t w) {
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int sh = M::kBit - 4 * p;
-    v[p] = ((sh >= 0 ? w << (sh & 31) : w >> (-sh & 31)) & M::kMask) | M::kBias;
+    v[p] = and_or(sh >= 0 ? w << (sh & 31) : w >> (-sh & 31), M::kMask, M::kBias);
   }
   return __builtin_bit_cast(typename M::v8, v);
 }
@@ -74,115 +102,173 @@ constexpr int kW4Block = 128;  // k per block
 __host__ __device__ inline int w4_gpb(int64_t group) { return group >= kW4Block ? 1 : static_cast<int>(kW4Block / group); }
 __host__ __device__ inline int64_t w4_block_bytes(int gpb) { return 1024 + 64 * gpb; }
 
-// A weight matrix as the kernels read it. GPB > 0: 4-bit, groups per block. GPB = 0: fp16/bf16, in
-// blocks of 64 k with element strides that cover row-major weights and both packed layouts.
-struct WeightView {
-  const void* w;
-  int64_t es;           // expert stride (4-bit: bytes)
-  int64_t s4, s1;       // 16 bits: strides of 64 rows and of 16 rows
-  int64_t ps;           // ... of the up half after the gate half
-  int64_t bs, hs;       // ... of 64 k and of 32 k
-  int64_t lr, lg;       // ... of a row in a fragment and of 8 k
-  int parts;            // 4-bit: slabs of one 16-column group (2: gate and up)
-  int nb;               // blocks of k
-};
+// One block of R slabs, as loaded.
+template <int R, int GPB>
+struct W4Block {
+  u32x4 w[R];
+  uint32_t m[R][GPB];
 
-// One lane's place in a 16-row slab's stream.
-template <typename T, int GPB>
-struct WeightPtr {
-  const T* p;
-  __device__ __forceinline__ void set(const WeightView& v, int64_t e, int slab, int part, int lane) {
-    p = static_cast<const T*>(v.w) + e * v.es + (slab >> 2) * v.s4 + (slab & 3) * v.s1 + part * v.ps +
-        (lane & 15) * v.lr + (lane >> 4) * v.lg;
-  }
-};
-
-template <typename T, int R, int NT, int GPB>
-struct Stage {
-  static constexpr int kFrags = GPB > 0 ? 4 : 2;  // 32-k steps of a block
-  static constexpr int kBlock = 32 * kFrags;
-  using V8 = typename Mfma16<T>::v8;
-  u32x4 w[R][GPB > 0 ? 1 : 2];
-  uint32_t m[R][GPB > 0 ? GPB : 1];
-  V8 x[NT][kFrags];
-
-  // 4-bit: base = the slab's first byte, uniform. The block's codes and its scales.
-  __device__ __forceinline__ void load_w4(int r, const uint8_t* base, int64_t block, int lane) {
-    const uint8_t* p = base + block * (1024 + 64 * GPB);
-    w[r][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + lane * 16));
-    const uint8_t* q = p + 1024 + (lane & 15) * (4 * GPB);
+  // slab: the slab's blocks. Buffer loads: the address is the resource, a scalar and one lane offset, so
+  // that no vector arithmetic goes into it.
+  __device__ __forceinline__ void load(int r, BufferRsrc slab, int block, int lane) {
+    const int at = block * (1024 + 64 * GPB);
+    w[r] = __builtin_amdgcn_raw_buffer_load_b128(slab, lane * 16, at, kPolicyNt);
+    const int mo = (lane & 15) * (4 * GPB);
     if constexpr (GPB == 4) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(q);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(slab, mo, at + 1024, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) m[r][i] = v[i];
     } else if constexpr (GPB == 2) {
-      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-      const u32x2 v = *reinterpret_cast<const u32x2*>(q);
+      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(slab, mo, at + 1024, 0);
       m[r][0] = v[0];
       m[r][1] = v[1];
     } else {
-      m[r][0] = *reinterpret_cast<const uint32_t*>(q);
+      m[r][0] = __builtin_amdgcn_raw_buffer_load_b32(slab, mo, at + 1024, 0);
     }
   }
-  // 16 bits: p = this lane's first element of the slab.
-  __device__ __forceinline__ void load_half(int r, const T* p, int64_t block, int64_t bs, int64_t hs) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      w[r][h & (GPB > 0 ? 0 : 1)] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + block * bs + h * hs));
-  }
-  // The tokens' k of a block: xrow = this lane's token row + 8 (lane / 16). K is a multiple of 32; steps
-  // past it re-read the last one (their weights have scale 0).
-  __device__ __forceinline__ void load_x(int nt, const T* xrow, int block, int K) {
-#pragma unroll
-    for (int f = 0; f < kFrags; ++f)
-      x[nt][f] = *reinterpret_cast<const V8*>(xrow + min(block * kBlock + 32 * f, K - 32));
-  }
 
-  // acc[nt][r] += the block's products.
-  __device__ __forceinline__ void compute(f32x4 (&acc)[NT][R]) const {
+  // acc[nt][r] += the block's products with the fragments x(nt, f).
+  template <typename T, int NT, typename X>
+  __device__ __forceinline__ void compute(X x, f32x4 (&acc)[NT][R]) const {
     using M = Mfma16<T>;
-    if constexpr (GPB == 0) {
+    using V8 = typename M::v8;
+    constexpr int FG = 4 / GPB;  // 32-k steps of a group
+    const V8 ones = __builtin_bit_cast(V8, u32x4{M::kOnes, M::kOnes, M::kOnes, M::kOnes});
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+    for (int g = 0; g < GPB; ++g) {
+      V8 xv[NT][FG];
+      f32x4 xs[NT];
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+      for (int nt = 0; nt < NT; ++nt) {
+        xs[nt] = zero;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            acc[nt][r] = M::run(x[nt][f], __builtin_bit_cast(V8, w[r][f]), acc[nt][r]);
-    } else {
-      constexpr int FG = 4 / GPB;  // steps of a group within the block
-      const V8 ones = __builtin_bit_cast(V8, u32x4{M::kOnes, M::kOnes, M::kOnes, M::kOnes});
-      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < FG; ++f) {
+          xv[nt][f] = __builtin_bit_cast(V8, x(nt, g * FG + f));
+          xs[nt] = M::run(xv[nt][f], ones, xs[nt]);
+        }
+      }
 #pragma unroll
-      for (int g = 0; g < GPB; ++g) {
-        f32x4 xs[NT];
+      for (int r = 0; r < R; ++r) {
+        f32x4 part[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) part[nt] = zero;
+#pragma unroll
+        for (int f = 0; f < FG; ++f) {
+          const V8 wv = w4_values<T>(w[r][g * FG + f]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) part[nt] = M::run(xv[nt][f], wv, part[nt]);
+        }
+        const float s = __builtin_bit_cast(float, m[r][g] & ~15u);
+        const float z = -16.0f - static_cast<float>(m[r][g] & 15u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          xs[nt] = zero;
 #pragma unroll
-          for (int f = 0; f < FG; ++f) xs[nt] = M::run(x[nt][g * FG + f], ones, xs[nt]);
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          f32x4 part[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) part[nt] = zero;
-#pragma unroll
-          for (int f = 0; f < FG; ++f) {
-            const V8 wv = w4_values<T>(w[r][0][g * FG + f]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) part[nt] = M::run(x[nt][g * FG + f], wv, part[nt]);
-          }
-          const float s = __builtin_bit_cast(float, m[r][g] & ~15u);
-          const float z = -16.0f - static_cast<float>(m[r][g] & 15u);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc[nt][r][i] = __builtin_fmaf(s, __builtin_fmaf(z, xs[nt][i], part[nt][i]), acc[nt][r][i]);
+          for (int i = 0; i < 4; ++i)
+            acc[nt][r][i] = __builtin_fmaf(s, __builtin_fmaf(z, xs[nt][i], part[nt][i]), acc[nt][r][i]);
+#if defined(__HIP_DEVICE_COMPILE__)
+          // the sums are made here: put off, the parts of every group and slab are live at once, and spill
+          asm volatile("" : "+v"(acc[nt][r]));
+#endif
         }
       }
     }
+  }
+};
+
+// A wave's tokens of one block: NT tiles of 4 XI rows. A load takes 4 rows' whole 256 bytes (a fragment's
+// own order would touch 64 lines an instruction: 2 us more at 16 tokens); the wave's piece of LDS turns
+// them into fragments. Row r's 16-byte piece p sits at p ^ r, so that neither side meets a bank twice.
+template <int NT, int XI>
+struct XBlock {
+  static constexpr int kPieces = 64 * XI * NT;  // of the wave's LDS
+  u32x4 x[NT * XI];
+
+  // off[i]: this lane's byte offset of row 4 i + lane / 16 and piece lane % 16 of block 0.
+  __device__ __forceinline__ void load(BufferRsrc rows, const int (&off)[NT * XI], int block, int k, int lane) {
+    const int past = nowhere(block * kW4Block + 8 * (lane & 15) >= k);
+#pragma unroll
+    for (int i = 0; i < NT * XI; ++i)
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, off[i] | past, block * (2 * kW4Block), 0);
+  }
+  __device__ __forceinline__ void put(u32x4* lds, int lane) const {
+    asm volatile("" ::: "memory");  // the reads of the block before are over: LDS answers a wave in order
+#pragma unroll
+    for (int i = 0; i < NT * XI; ++i) {
+      const int r = 4 * i + (lane >> 4);
+      lds[16 * r + ((lane & 15) ^ (r & 15))] = x[i];
+    }
+    asm volatile("" ::: "memory");
+  }
+  static __device__ __forceinline__ u32x4 frag(const u32x4* lds, int nt, int f, int lane) {
+    const int r = lane & (4 * XI - 1);
+    return lds[16 * (16 * nt + r) + ((4 * f + (lane >> 4)) ^ r)];
+  }
+};
+
+// A wave's stream of items [first, end), D of them in flight.
+template <typename S, int D, typename Issue, typename Consume>
+__device__ __forceinline__ void stream(int first, int end, Issue issue, Consume consume) {
+  if (first >= end) return;
+  S ring[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    issue(ring[d], first + d);
+    __builtin_amdgcn_sched_barrier(0);  // in the ring's order, the oldest consumed first
+  }
+  int j = first;
+  for (; j + D < end; j += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      consume(ring[d], j + d);
+      issue(ring[d], j + D + d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (j + d < end) consume(ring[d], j + d);
+}
+
+// A 16-bit weight matrix of experts, in blocks of 64 k, by element strides that cover row-major weights
+// and both packed layouts; or a packed 4-bit one (w, es in bytes, nb).
+struct WeightView {
+  const void* w;
+  int64_t es;       // expert stride
+  int64_t s4, s1;   // 64 rows and 16 rows
+  int64_t ps;       // the up half after the gate half
+  int64_t bs, hs;   // 64 k and 32 k
+  int64_t lr, lg;   // a row in a fragment and 8 k
+  int nb;           // blocks of k
+};
+
+template <typename T>
+__device__ __forceinline__ const T* half_slab(const WeightView& v, int64_t e, int slab, int part, int lane) {
+  return static_cast<const T*>(v.w) + e * v.es + (slab >> 2) * v.s4 + (slab & 3) * v.s1 + part * v.ps +
+         (lane & 15) * v.lr + (lane >> 4) * v.lg;
+}
+
+// A block of R slabs of 16-bit weights and its 16 tokens, in fragment order.
+template <typename T, int R>
+struct HalfStage {
+  using V8 = typename Mfma16<T>::v8;
+  u32x4 w[R][2];
+  V8 x[2];
+
+  __device__ __forceinline__ void load(int r, const T* p, int64_t block, int64_t bs, int64_t hs) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[r][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + block * bs + h * hs));
+  }
+  __device__ __forceinline__ void load_x(const T* xrow, int block) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) x[h] = *reinterpret_cast<const V8*>(xrow + block * 64 + 32 * h);
+  }
+  __device__ __forceinline__ void compute(f32x4 (&acc)[1][R]) const {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc[0][r] = Mfma16<T>::run(x[h], __builtin_bit_cast(V8, w[r][h]), acc[0][r]);
   }
 };
 

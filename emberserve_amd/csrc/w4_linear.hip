@@ -2,19 +2,16 @@
 //   out[t, n] = round(sum_k x[t, k] s[n, g(k)] (q[n, k] - z[n, g(k)]) + bias[n])
 // and the dense MLP's gate_up form, round(silu(gate) * up), over the packed layout of w4.h.
 //
-// What bounds it: the weights' bytes (N K / 2 and the scales), read once. A wave holds R slabs of 16
-// weight rows against up to 64 tokens, so a block's codes are loaded once (one 16-byte non-temporal
-// load per lane and slab) and turned into MFMA operands in registers; nothing goes through LDS but
-// the sums of the waves that share a slab's k.
+// What bounds it: the weights' bytes (N K / 2 and the scales), read once, and what a CU can issue of loads:
+// the tokens are loaded again by every workgroup (from L2). A wave holds 1 to 4 slabs of 16 weight rows
+// against up to 32 tokens; a block of 128 k of a slab is one 16-byte non-temporal load a lane, turned into
+// MFMA operands in registers.
 #include <algorithm>
 
 #include "w4.h"
 
 namespace ember {
 namespace {
-
-constexpr int kW4Waves = 8;
-constexpr int kW4Tokens = 64;  // tokens of one pass over the weights
 
 struct W4Args {
   const void* x;
@@ -25,151 +22,172 @@ struct W4Args {
   int64_t os;
   int T, K, N;   // N: columns of out
   int slabs, nb; // slabs of the packed weight (gate_up: twice the column slabs), blocks of k
-  int wk;        // waves that share a slab's k: 1, 2, 4 or 8
+  int groups;    // sets of R slabs
+  int tiles;     // sets of 16 NT tokens
   int gate_up;
 };
 
-// NT token tiles of 16, R slabs a wave, D blocks in flight.
-template <typename T, int NT, int R, int GPB, int D>
-__global__ void __launch_bounds__(kW4Waves * kWave)
+constexpr int kXcds = 8;
+
+// A workgroup holds R slabs against NT tiles of 16 tokens (XI < 4: of 4 XI); its waves share k, block by
+// block. D blocks in flight a wave.
+template <typename T, int R, int GPB, int NT, int XI, int D, int MAXW>
+__global__ void __launch_bounds__(MAXW * kWave)
 k_w4_linear(W4Args a) {
-  using S = Stage<T, R, NT, GPB>;
-  extern __shared__ __attribute__((aligned(16))) float red[];  // wk > 1: [wave][NT * R][lane] x 4
+  using X = XBlock<NT, XI>;
+  constexpr int P = X::kPieces > 64 * R * NT ? X::kPieces : 64 * R * NT;
+  extern __shared__ __attribute__((aligned(16))) u32x4 lds[];  // [wave][P]: a block's tokens, then the sums
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kpart = wave & (a.wk - 1);
-  const int slab0 = (blockIdx.x * (kW4Waves / a.wk) + wave / a.wk) * R;
-  const int tok0 = blockIdx.y * kW4Tokens;
-  const uint8_t* base[R];
+  const int wk = blockDim.x >> 6;
+  // the tiles of a slab group on one XCD, next to each other: its L2 holds the weights for them
+  const int per = kXcds * a.tiles;
+  const int tile = blockIdx.x % per / kXcds;
+  const int group = blockIdx.x / per * kXcds + blockIdx.x % kXcds;
+  if (group >= a.groups) return;
+  const int slab0 = group * R, tok0 = 16 * NT * tile;
+  const int rows = min(a.T - tok0, 16 * NT);
+  const BufferRsrc xr = buffer(static_cast<const T*>(a.x) + static_cast<int64_t>(tok0) * a.xs,
+                               static_cast<int>(((rows - 1) * a.xs + a.K) * 2));
+  int off[NT * XI];
+#pragma unroll
+  for (int i = 0; i < NT * XI; ++i)
+    off[i] = min(4 * i + (lane >> 4), rows - 1) * static_cast<int>(a.xs) * 2 + 16 * (lane & 15);
+  const int64_t slab_bytes = a.nb * w4_block_bytes(GPB);
+  BufferRsrc base[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    base[r] = a.w + static_cast<int64_t>(min(slab0 + r, a.slabs - 1)) * a.nb * w4_block_bytes(GPB);
-  const T* xrow[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-    xrow[nt] = static_cast<const T*>(a.x) + static_cast<int64_t>(min(tok0 + 16 * nt + (lane & 15), a.T - 1)) * a.xs +
-               8 * (lane >> 4);
-  S ring[D];
+    base[r] = buffer(a.w + min(slab0 + r, a.slabs - 1) * slab_bytes, static_cast<int>(slab_bytes));
+
+  struct Stage {
+    W4Block<R, GPB> w;
+    X x;
+  };
+  u32x4* const mine = lds + wave * P;
   f32x4 acc[NT][R];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[nt][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int nj = slab0 < a.slabs && kpart < a.nb ? (a.nb - kpart + a.wk - 1) / a.wk : 0;
-  auto issue = [&](S& st, int j) {
-    const int b = min(kpart + j * a.wk, a.nb - 1);
+  stream<Stage, D>(
+      0, wave < a.nb ? (a.nb - wave + wk - 1) / wk : 0,
+      [&](Stage& g, int j) {
+        const int b = min(wave + j * wk, a.nb - 1);
 #pragma unroll
-    for (int r = 0; r < R; ++r) st.load_w4(r, base[r], b, lane);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) st.load_x(nt, xrow[nt], b, a.K);
-  };
-  if (nj > 0) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      issue(ring[d], d);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    int j0 = 0;
-    for (; j0 + D < nj; j0 += D) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        ring[d].compute(acc);
-        issue(ring[d], j0 + D + d);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (j0 + d < nj) ring[d].compute(acc);
-  }
+        for (int r = 0; r < R; ++r) g.w.load(r, base[r], b, lane);
+        g.x.load(xr, off, b, a.K, lane);
+      },
+      [&](const Stage& g, int) {
+        g.x.put(mine, lane);
+        g.w.template compute<T, NT>([&](int nt, int f) { return X::frag(mine, nt, f, lane); }, acc);
+      });
 
   // lane: column l % 16 of its slab, tokens 16 nt + 4 (l / 16) + i
   auto emit = [&](int nt, int slab, f32x4 v, f32x4 up) {
     const int col = (a.gate_up ? slab >> 1 : slab) * 16 + (lane & 15);
-    if (col >= a.N) return;
+    if (slab >= a.slabs || col >= a.N) return;
     const float bias = a.bias != nullptr ? to_f32(static_cast<const T*>(a.bias)[col]) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int tok = tok0 + 16 * nt + 4 * (lane >> 4) + i;
-      if (tok >= a.T) continue;
+      const int tok = 16 * nt + 4 * (lane >> 4) + i;
+      if (tok >= rows) continue;
       const float y = a.gate_up ? silu_mul(v[i], up[i]) : v[i] + bias;
-      static_cast<T*>(a.out)[static_cast<int64_t>(tok) * a.os + col] = from_f32<T>(y);
+      static_cast<T*>(a.out)[static_cast<int64_t>(tok0 + tok) * a.os + col] = from_f32<T>(y);
     }
   };
-  const int step = a.gate_up ? 2 : 1;  // gate and up slabs alternate; R is even then
-  if (a.wk == 1) {
+  if (wk == 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if ((r % 2 == 0 || step == 1) && slab0 + r < a.slabs) emit(nt, slab0 + r, acc[nt][r], acc[nt][R > 1 ? (r | 1) : 0]);
+        if (r % 2 == 0 || !a.gate_up) emit(nt, slab0 + r, acc[nt][r], acc[nt][R > 1 ? r | 1 : r]);
     return;
   }
-  f32x4* lds = reinterpret_cast<f32x4*>(red);
+  // the waves take the tiles (gate and up together) in turn, summing the waves' shares of k in order
+  f32x4* const red = reinterpret_cast<f32x4*>(lds);
+  asm volatile("" ::: "memory");
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int r = 0; r < R; ++r) lds[(wave * NT * R + nt * R + r) * kWave + lane] = acc[nt][r];
+    for (int r = 0; r < R; ++r) red[wave * P + (nt * R + r) * kWave + lane] = acc[nt][r];
   __syncthreads();
-  // the waves of a slab take its tiles in turn, summing the k parts in order
-  const int first = wave - kpart;
-  auto total = [&](int tile) {
-    f32x4 v = lds[(first * NT * R + tile) * kWave + lane];
-    for (int q = 1; q < a.wk; ++q) v += lds[((first + q) * NT * R + tile) * kWave + lane];
+  auto total = [&](int t) {
+    f32x4 v = red[t * kWave + lane];
+    for (int q = 1; q < wk; ++q) v += red[q * P + t * kWave + lane];
     return v;
   };
-  for (int tile = kpart * step; tile < NT * R; tile += a.wk * step) {
-    const int slab = slab0 + tile % R;
-    if (slab >= a.slabs) continue;
-    const f32x4 v = total(tile);
-    emit(tile / R, slab, v, a.gate_up ? total(tile + 1) : v);
+  const int step = a.gate_up ? 2 : 1;
+  for (int t = wave * step; t < NT * R; t += wk * step) {
+    const f32x4 v = total(t);
+    emit(t / R, slab0 + t % R, v, a.gate_up ? total(t + 1) : v);
   }
 }
 
-template <typename T, int NT, int R, int GPB, int D>
-int w4_launch(const W4Args& a, hipStream_t stream) {
-  const int groups = static_cast<int>(cdiv(a.slabs, R));
-  const dim3 grid(static_cast<unsigned>(cdiv(groups, kW4Waves / a.wk)), static_cast<unsigned>(cdiv(a.T, kW4Tokens)));
-  const size_t lds = a.wk > 1 ? size_t(kW4Waves) * NT * R * kWave * 16 : 0;
-  k_w4_linear<T, NT, R, GPB, D><<<grid, kW4Waves * kWave, lds, stream>>>(a);
+template <typename T, int R, int GPB, int NT, int XI, int D, int MAXW>
+int w4_launch(W4Args a, hipStream_t stream) {
+  const int64_t cus = std::max(1, device_cu_count());
+  a.groups = static_cast<int>(cdiv(a.slabs, R));
+  a.tiles = static_cast<int>(cdiv(a.T, 16 * NT));
+  const int64_t grid = cdiv(a.groups, kXcds) * kXcds * a.tiles;
+  // Waves along k: 7 or more a CU, each with at least a block or two. Measured (us at 1 | 2 | 4 | 8 | 16):
+  // Qwen2.5-7B down, 2 tokens (224 slabs, 148 blocks) ... | 12.6 | 11.8 | 13.6; Qwen3-8B head, 16 tokens
+  // (2374 sets) 70.4 | 75.6 | 76.7.
+  int wk = 1;
+  while (wk < MAXW && grid * wk < 7 * cus && 2 * wk < a.nb) wk *= 2;
+  const size_t lds = size_t(wk) * 16 * std::max(XBlock<NT, XI>::kPieces, 64 * R * NT);
+  k_w4_linear<T, R, GPB, NT, XI, D, MAXW><<<dim3(static_cast<unsigned>(grid)), wk * kWave, lds, stream>>>(a);
   return launch_status();
 }
 
-// Slabs a wave and waves along k, from sizes: see w4_run.
+// Slabs a workgroup: more of them share a block's tokens, whose loads take about as long as one slab's, but
+// fewer workgroups fill the chip. The number with the shortest rounds. Measured (us at 1 | 2 | 4 slabs):
+// 256 slabs x 4096, 16 tokens 6.8 | 7.8 | 11.1; 384 x 4096, 16 tokens 9.2 | 8.0 | 11.3, 64 tokens 18.2 | 16.7
+// | 12.5; gate_up 1536 x 4096, 16 tokens 2 | 4: 18.3 | 21.9, 64 tokens 35.1 | 31.6.
+int w4_slabs(const W4Args& a, int tokens) {
+  const int64_t cus = std::max(1, device_cu_count()), tiles = cdiv(a.T, tokens);
+  int best = 0;
+  int64_t least = 0;
+  for (int r = a.gate_up ? 2 : 1; r <= 4; r *= 2) {
+    const int64_t cost = cdiv(cdiv(a.slabs, r) * tiles, cus) * (r + 1);
+    if (best == 0 || cost < least) {
+      best = r;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+// Token tiles, slabs and depth by size. Two tiles a wave from 17 tokens: the codes are turned into operands
+// once for both (gate_up of Qwen2.5-7B, 27 tokens, 35.6 us with one tile a wave, 28.8 with two). Up to 4
+// and 8 tokens a block's tokens are one and two loads instead of four, and the ring is deeper.
 template <typename T, int GPB>
-int w4_pick(W4Args a, int r, hipStream_t stream) {
-  const int nt = a.T <= 16 ? 1 : (a.T <= 32 ? 2 : 4);
-  if (nt == 1) {
-    if (r == 1) return w4_launch<T, 1, 1, GPB, 4>(a, stream);
-    if (r == 2) return w4_launch<T, 1, 2, GPB, 4>(a, stream);
-    return w4_launch<T, 1, 4, GPB, 3>(a, stream);
+int w4_pick(const W4Args& a, hipStream_t stream) {
+  if (a.T <= 4) {
+    if (!a.gate_up) return w4_launch<T, 1, GPB, 1, 1, GPB == 4 ? 6 : 8, 16>(a, stream);
+    return w4_launch<T, 2, GPB, 1, 1, GPB == 4 ? 3 : 4, 16>(a, stream);
   }
-  if (nt == 2) {
-    if (r == 1) return w4_launch<T, 2, 1, GPB, 3>(a, stream);
-    if (r == 2) return w4_launch<T, 2, 2, GPB, 3>(a, stream);
-    return w4_launch<T, 2, 4, GPB, 2>(a, stream);
+  const int r = w4_slabs(a, a.T <= 16 ? 16 : 32);
+  if (a.T <= 8) {
+    if (r == 1) return w4_launch<T, 1, GPB, 1, 2, 4, 16>(a, stream);
+    if (r == 2) return w4_launch<T, 2, GPB, 1, 2, 4, 8>(a, stream);
+    return w4_launch<T, 4, GPB, 1, 2, 3, 8>(a, stream);
   }
-  if (r == 1) return w4_launch<T, 4, 1, GPB, 2>(a, stream);
-  if (r == 2) return w4_launch<T, 4, 2, GPB, 2>(a, stream);
-  return w4_launch<T, 4, 4, GPB, 1>(a, stream);
+  if (a.T <= 16) {
+    if (r == 1) return w4_launch<T, 1, GPB, 1, 4, GPB == 1 ? 4 : 3, 16>(a, stream);
+    if (r == 2) return w4_launch<T, 2, GPB, 1, 4, 4, 8>(a, stream);
+    return w4_launch<T, 4, GPB, 1, 4, 3, 8>(a, stream);
+  }
+  if (r == 1) return w4_launch<T, 1, GPB, 2, 4, 3, 8>(a, stream);
+  if (r == 2) return w4_launch<T, 2, GPB, 2, 4, 2, 8>(a, stream);
+  return w4_launch<T, 4, GPB, 2, 4, 2, 8>(a, stream);
 }
 
 template <typename T>
-int w4_run(W4Args a, int gpb, hipStream_t stream) {
-  const int64_t waves = 8 * std::max(1, device_cu_count());
-  // Slabs a wave: more of them share a block's tokens; as many as leave the chip its waves.
-  int r = a.gate_up ? 2 : 1;
-  const int most = a.T <= 16 ? 2 : 4;
-  while (r < most && a.slabs / (2 * r) >= waves) r *= 2;
-  int wk = 1;
-  while (wk < kW4Waves && cdiv(a.slabs, r) * wk < waves && 2 * wk <= a.nb) wk *= 2;
-  const int nt = a.T <= 16 ? 1 : (a.T <= 32 ? 2 : 4);
-  if (wk > 1 && nt * r > 8) wk = 1;  // 64 KiB of LDS
-  a.wk = wk;
+int w4_run(const W4Args& a, int gpb, hipStream_t stream) {
   switch (gpb) {
-    case 1: return w4_pick<T, 1>(a, r, stream);
-    case 2: return w4_pick<T, 2>(a, r, stream);
-    default: return w4_pick<T, 4>(a, r, stream);
+    case 1: return w4_pick<T, 1>(a, stream);
+    case 2: return w4_pick<T, 2>(a, stream);
+    default: return w4_pick<T, 4>(a, stream);
   }
 }
 
@@ -186,12 +204,12 @@ int w4_call(const void* x, int64_t xs, const void* packed, int64_t group, int dt
             int64_t rows, int gate_up, const void* bias, void* out, int64_t os, void* stream) {
   if (tokens == 0 && sizes_ok(rows, k, group)) return EMBER_OK;
   if (x == nullptr || packed == nullptr || out == nullptr || tokens < 0 || tokens > (int64_t(1) << 21) ||
-      !sizes_ok(rows, k, group) || (dtype != EMBER_F16 && dtype != EMBER_BF16) || os < 0 || xs < 0)
+      !sizes_ok(rows, k, group) || xs > (int64_t(1) << 24) || (dtype != EMBER_F16 && dtype != EMBER_BF16) || os < 0 || xs < 0)
     return EMBER_EINVAL;
   if (!aligned16(x) || !aligned16(packed) || xs % 8 != 0) return EMBER_EALIGN;
   W4Args a{x, xs, static_cast<const uint8_t*>(packed), bias, out, os, static_cast<int>(tokens), static_cast<int>(k),
            static_cast<int>(rows), static_cast<int>(cdiv(rows, 16)) * (gate_up ? 2 : 1),
-           static_cast<int>(cdiv(k, kW4Block)), 1, gate_up};
+           static_cast<int>(cdiv(k, kW4Block)), 0, 1, gate_up};
   const int gpb = w4_gpb(group);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == EMBER_F16 ? w4_run<_Float16>(a, gpb, s) : w4_run<__bf16>(a, gpb, s);

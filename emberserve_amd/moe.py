@@ -579,7 +579,7 @@ def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tens
         return fused_moe_torch(x, topk_ids, topk_weights, a, b)
     if not w4 and (H % 64 or I % 64):
         raise ValueError(f"fused_moe: H and I must be multiples of 64, got {H} and {I}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) > 1 << 23 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
     out = torch.empty((n, H), dtype=x.dtype, device=x.device)

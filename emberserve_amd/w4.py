@@ -31,6 +31,7 @@ from . import _lib
 from .ops import _launch, fused_enabled
 
 SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
+MAX_ROW_STRIDE = 1 << 24  # elements: a tile of tokens is addressed with 32-bit offsets
 
 
 def quantize_w4(weight: Tensor, group_size: int = 128, *, symmetric: bool = True) -> tuple[Tensor, Tensor, Tensor | None]:
@@ -183,7 +184,7 @@ def _check(what: str, x: Tensor, weight: PackedW4, gate_up: bool) -> None:
 def _rows(x: Tensor) -> Tensor:
     """x as [T, K] rows that the kernels can read: unit inner stride, 16-byte aligned."""
     x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) > MAX_ROW_STRIDE or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 

@@ -679,7 +679,7 @@ int ember_moe_layer(const void* x, int64_t x_row_stride, const void* topk_ids, i
 
 /* ember_moe_layer over experts packed by ember_w4_pack_weight: the gate_up weight with gate_up, rows =
  * inter, k = hidden; the down weight with rows = hidden, k = inter. hidden and inter multiples of 32
- * that their groups divide. */
+ * that their groups divide, hidden at most 16384. */
 int ember_moe_layer_w4(const void* x, int64_t x_row_stride, const void* topk_ids, int id_bytes,
                        const void* topk_weights, int weight_dtype, int64_t num_tokens, int64_t top_k,
                        const void* packed_gate_up, int64_t gate_up_group, const void* packed_down, int64_t down_group,
