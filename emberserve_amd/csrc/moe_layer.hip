@@ -32,7 +32,7 @@ constexpr int kMlMaxSplits = 16;
 constexpr int kMlTokenLds = 128 << 10;      // a group's tokens, 4-bit weights
 constexpr int kMlMaxHiddenW4 = kMlTokenLds / 8;  // ... of four rows
 constexpr int kUpWaves = 4, kDownWaves = 8;      // 16-bit weights
-constexpr int kUpWavesW4 = 8, kDownWavesW4 = 4;  // 4-bit weights
+constexpr int kUpWavesW4 = 8, kShareWavesW4 = 4, kDownWavesW4 = 4;  // 4-bit weights
 constexpr int kDownSlabsW4 = 2;                  // slabs of 16 columns a wave of theirs holds
 
 struct MlArgs {
@@ -46,7 +46,7 @@ struct MlArgs {
   WeightView w1, w2;
   void* act;          // [A][I]
   int* gexpert;       // [0]: number of groups, then each group's expert
-  int* glist;         // [group][16] assignments, -1: none
+  int16_t* glist;     // [group][16] assignments, -1: none
   float* part;        // the second kernel's partials
   uint32_t* counters; // one per slab set of the second kernel
   void* out;
@@ -72,6 +72,7 @@ __device__ __forceinline__ int lanes_below(uint64_t mask, int lane) {
 template <int W>
 struct GroupLds {
   int count[kMlMaxExperts];
+  int16_t expert[kMlMaxAssign];  // of each assignment, -1: none
   int list[W][kMlTile];
 };
 
@@ -103,12 +104,14 @@ __device__ __forceinline__ int find_group(const MlArgs& a, int u, bool lead, boo
       asm volatile("" ::: "memory");
     }
   } else {
-    for (int e = threadIdx.x; e < a.E; e += W * kWave) g.count[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) g.count[e] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.A; i += W * kWave) {
+    for (int i = threadIdx.x; i < a.A; i += blockDim.x) {
       const int64_t e = ml_id(a, i);
-      if (e >= 0 && e < a.E) atomicAdd(&g.count[e], 1);
+      const bool ok = e >= 0 && e < a.E;
+      if (ok) atomicAdd(&g.count[e], 1);
       else bad |= e != -1;
+      g.expert[i] = ok ? static_cast<int16_t>(e) : static_cast<int16_t>(-1);
     }
     __syncthreads();
     int rank = 0;  // every wave finds the same
@@ -133,7 +136,7 @@ __device__ __forceinline__ int find_group(const MlArgs& a, int u, bool lead, boo
       asm volatile("" ::: "memory");
       int seen = 0;
       for (int i0 = 0; i0 < a.A; i0 += kWave) {
-        const bool mine = i0 + lane < a.A && ml_id(a, i0 + lane) == expert;
+        const bool mine = i0 + lane < a.A && g.expert[i0 + lane] == expert;
         const uint64_t m = __ballot(mine);
         const int at = seen + lanes_below(m, lane) - rank;
         if (mine && at >= 0 && at < a.tile) list[at] = i0 + lane;
@@ -146,7 +149,7 @@ __device__ __forceinline__ int find_group(const MlArgs& a, int u, bool lead, boo
   if (lead && threadIdx.x == 0) a.gexpert[0] = groups;
   expert = __builtin_amdgcn_readfirstlane(expert);
   if (expert >= 0 && record && threadIdx.x < kMlTile) {
-    a.glist[u * kMlTile + threadIdx.x] = list[threadIdx.x];
+    a.glist[u * kMlTile + threadIdx.x] = static_cast<int16_t>(list[threadIdx.x]);
     if (threadIdx.x == 0) a.gexpert[1 + u] = expert;
   }
   return expert;
@@ -212,7 +215,7 @@ k_moe_layer_up_w4(MlArgs a) {
   if (expert < 0) return;
   const int* list = group.list[wave];
   const int nb = a.w1.nb;
-  const int64_t slab_bytes = nb * w4_block_bytes(GPB);
+  const int64_t slab_bytes = w4_slab_bytes(nb, GPB);
   const uint8_t* w = static_cast<const uint8_t*>(a.w1.w) + expert * a.w1.es;
 
   // item j of this wave: block b of slab s, both in steps
@@ -246,7 +249,7 @@ k_moe_layer_up_w4(MlArgs a) {
       const int id = list[4 * i + (lane >> 4)];
       off[i] = (id >= 0 ? id : list[0]) / a.top_k * static_cast<int>(a.xs) * 2 + 16 * (lane & 15);
     }
-    for (int b = wave; b < nb; b += kUpWavesW4) {
+    for (int b = wave; b < nb; b += static_cast<int>(blockDim.x) / kWave) {
       X x;
       x.load(xr, off, b, a.H, lane);
       x.put(tokens + b * X::kPieces, lane);
@@ -260,7 +263,7 @@ k_moe_layer_up_w4(MlArgs a) {
         const int b = b0 + ld.j * b_step;
         const uint8_t* at = w + 2 * s * slab_bytes;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) st.load(r, buffer(at + r * slab_bytes, static_cast<int>(slab_bytes)), b, lane);
+        for (int r = 0; r < 2; ++r) st.load(r, buffer(at + r * slab_bytes, static_cast<int>(slab_bytes)), b, nb, lane);
         if (++ld.j == blocks) {
           ld.j = 0;
           ++ld.s;
@@ -287,7 +290,7 @@ k_moe_layer_up_w4(MlArgs a) {
   __syncthreads();
   if (wave != 0) return;
   f32x4 g = red[lane], up = red[kWave + lane];
-  for (int q = 1; q < kUpWavesW4; ++q) {
+  for (int q = 1; q < a.wk; ++q) {
     g += red[2 * q * kWave + lane];
     up += red[(2 * q + 1) * kWave + lane];
   }
@@ -312,7 +315,7 @@ struct Down {
     all = lds;  // [wave][N][kCols]
     sums = all + wave * a.N * kCols;
     wts = all + W * a.N * kCols;
-    lists = reinterpret_cast<int16_t*>(wts + a.A);
+    lists = reinterpret_cast<int16_t*>(wts + (a.A + 3) / 4 * 4);
     experts = lists + G * kMlTile;
     for (int i = lane; i < a.N * kCols; i += kWave) sums[i] = 0.f;
     for (int i = threadIdx.x; i < a.A; i += W * kWave) {
@@ -322,7 +325,8 @@ struct Down {
       else w = to_f32(static_cast<const __bf16*>(a.weights)[i]);
       wts[i] = w;
     }
-    for (int i = threadIdx.x; i < G * kMlTile; i += W * kWave) lists[i] = static_cast<int16_t>(a.glist[i]);
+    for (int i = threadIdx.x; i < G * kMlTile / 8; i += W * kWave)
+      reinterpret_cast<u32x4*>(lists)[i] = reinterpret_cast<const u32x4*>(a.glist)[i];
     for (int i = threadIdx.x; i < G; i += W * kWave) experts[i] = static_cast<int16_t>(a.gexpert[1 + i]);
     __syncthreads();
   }
@@ -436,7 +440,7 @@ k_moe_layer_down(MlArgs a) {
 }
 
 template <typename T, int GPB, int XI>
-__global__ void __launch_bounds__(kDownWavesW4 * kWave)
+__global__ void __launch_bounds__(kDownWavesW4 * kWave, 4)
 k_moe_layer_down_w4(MlArgs a) {
   using X = XBlock<1, XI>;
   constexpr int R = kDownSlabsW4;
@@ -445,7 +449,7 @@ k_moe_layer_down_w4(MlArgs a) {
   __shared__ int last;
   Down<T, R, kDownWavesW4> d(a, lds);
   const int nb = a.w2.nb, i0 = d.item(nb, 0), i1 = d.item(nb, 1);
-  const int64_t slab_bytes = nb * w4_block_bytes(GPB);
+  const int64_t slab_bytes = w4_slab_bytes(nb, GPB);
   const BufferRsrc ar = buffer(a.act, a.A * a.I * 2);
   f32x4 acc[1][R];
 #pragma unroll
@@ -459,7 +463,7 @@ k_moe_layer_down_w4(MlArgs a) {
 #pragma unroll
   for (int i = 0; i < XI; ++i) off[i] = 0;
   const uint8_t* w = nullptr;
-  stream<Stage, 4>(
+  stream<Stage, XI == 1 ? 4 : (XI == 2 ? 3 : 2)>(
       i0, i1,
       [&](Stage& st, int item) {
         const int it = min(item, i1 - 1);
@@ -473,7 +477,7 @@ k_moe_layer_down_w4(MlArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
-          st.w.load(r, buffer(w + r * slab_bytes, static_cast<int>(slab_bytes)), b, d.lane);
+          st.w.load(r, buffer(w + r * slab_bytes, static_cast<int>(slab_bytes)), b, nb, d.lane);
         st.x.load(ar, off, b, a.I, d.lane);
       },
       [&](const Stage& st, int item) {
@@ -486,12 +490,11 @@ k_moe_layer_down_w4(MlArgs a) {
 }
 
 // Assignments of a group: 16 rows are one MFMA tile; 4-bit weights stream fast enough that 16 rows of
-// tokens in LDS would cost them occupancy, so their groups are as small as holds twice the mean, and
-// take at most kMlTokenLds bytes.
+// tokens in LDS would cost them occupancy, so their groups are as small as holds nearly every expert's
+// share of a mean of 2.5 and of 5, and take at most kMlTokenLds bytes.
 int group_tile(int64_t A, int64_t E, int64_t H, bool w4) {
   if (!w4) return kMlTile;
-  const int64_t mean2 = 2 * cdiv(A, std::min(A, E));
-  int tile = mean2 <= 4 ? 4 : (mean2 <= 8 ? 8 : 16);
+  int tile = 2 * A <= 5 * E ? 4 : (A <= 5 * E ? 8 : 16);
   while (tile * cdiv(H, kW4Block) * kW4Block * 2 > kMlTokenLds) tile /= 2;
   return tile;
 }
@@ -520,7 +523,7 @@ MlLayout ml_layout(int64_t N, int64_t top_k, int64_t E, int64_t H, int64_t I) {
   l.act = 0;
   l.gexpert = up(A * I * 2);
   l.glist = l.gexpert + up(4 * (g + 1));
-  l.part = l.glist + up(4 * kMlTile * g);
+  l.part = l.glist + up(2 * kMlTile * g);
   l.partial = l.part + up(kMlMaxSplits * N * H * 4);
   l.counters = up(H / 16 * 4);
   return l;
@@ -532,7 +535,7 @@ bool ml_sizes_ok(int64_t N, int64_t top_k, int64_t E, int64_t H, int64_t I) {
 }
 
 size_t down_lds(const MlArgs& a, int waves, int cols) {
-  return 4 * (size_t(waves) * a.N * cols + a.A) + 2 * size_t(max_groups(a.A, a.E, a.tile)) * (kMlTile + 1) + 16;
+  return 4 * (size_t(waves) * a.N * cols + a.A + 3) + 2 * size_t(max_groups(a.A, a.E, a.tile)) * (kMlTile + 1) + 16;
 }
 
 template <typename T>
@@ -552,17 +555,19 @@ template <typename T, int GPB, int XI>
 int ml_up_w4(MlArgs a, hipStream_t s) {
   a.slabs = a.I / 16;
   const int64_t groups = max_groups(a.A, a.E, a.tile), cus = std::max(1, device_cu_count());
-  // whole slabs a wave once they fill the chip twice over; until then the waves share a slab's k
+  // Whole slabs a wave once they fill the chip twice over; until then the waves share a slab's k: four of
+  // them, so that a token's workgroups are on the chip at once (Moonlight's 528: 8 waves each took two turns)
   const bool whole = groups * a.slabs >= 2 * kUpWavesW4 * cus;
-  a.wk = whole ? 1 : kUpWavesW4;
-  a.per_wg = whole ? kUpWavesW4 : 1;
-  const size_t lds = 16 * (size_t(a.w1.nb) * XBlock<1, XI>::kPieces + (whole ? 0 : kUpWavesW4 * 2 * kWave));
+  const int waves = whole ? kUpWavesW4 : kShareWavesW4;
+  a.wk = whole ? 1 : waves;
+  a.per_wg = whole ? waves : 1;
+  const size_t lds = 16 * (size_t(a.w1.nb) * XBlock<1, XI>::kPieces + (whole ? 0 : waves * 2 * kWave));
   auto kernel = k_moe_layer_up_w4<T, GPB, XI>;
   if (lds > 65536 - sizeof(GroupLds<kUpWavesW4>) &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                           static_cast<int>(lds)) != hipSuccess)
     return EMBER_ENODEV;
-  kernel<<<dim3(static_cast<unsigned>(groups * cdiv(a.slabs, a.per_wg))), kUpWavesW4 * kWave, lds, s>>>(a);
+  kernel<<<dim3(static_cast<unsigned>(groups * cdiv(a.slabs, a.per_wg))), waves * kWave, lds, s>>>(a);
   return launch_status();
 }
 
@@ -638,7 +643,7 @@ int ml_call(const MlCall& c, const WeightView& w1, const WeightView& w2, int gpb
   a.w2 = w2;
   a.act = ws + l.act;
   a.gexpert = reinterpret_cast<int*>(ws + l.gexpert);
-  a.glist = reinterpret_cast<int*>(ws + l.glist);
+  a.glist = reinterpret_cast<int16_t*>(ws + l.glist);
   a.part = reinterpret_cast<float*>(ws + l.part);
   a.counters = reinterpret_cast<uint32_t*>(ws + c.workspace_bytes - l.counters);
   a.out = c.out;

@@ -16,14 +16,15 @@
 // 2 bits of fp32's 24; the scale is applied to the fp32 difference, once per group. No product is
 // rounded to 16 bits. An infinite x gives NaN (inf - inf) where the formula's sum would be infinite.
 //
-// Packed layout: per expert, slabs of 16 rows (gate_up: gate slab 0, up slab 0, gate slab 1, ...),
-// each a run of ceil(K / 128) blocks of 1024 + 64 gpb bytes, gpb = 128 / group (1 from 128 on):
+// Packed layout: per expert, slabs of 16 rows (gate_up: gate slab 0, up slab 0, gate slab 1, ...). A slab
+// is nb = ceil(K / 128) blocks of 1 KiB of codes, then the scales of all blocks, rounded up to 128 bytes:
 //   block[lane][f]: 32-bit word of the codes of row lane % 16 at k = 128 b + 32 f + 8 (lane / 16) + j,
 //                   j = 0..7 at bits 4 (j / 2) + 16 (j % 2)          (lane < 64, f < 4)
-//   then [row][gpb]: the group's scale as fp32 bits (exact from fp16 or bf16, whose low 13 mantissa
-//                   bits are zero) with z in the low four bits.
-// One 16-byte load per lane is a whole block's codes, and a slab is one contiguous stream. Groups
-// past K and rows past N have scale 0.
+//   scales[block][row][gpb]: gpb = 128 / group groups a block (1 from 128 on), each the scale as fp32 bits
+//                   (exact from fp16 or bf16, whose low 13 mantissa bits are zero) with z in the low four.
+// One 16-byte load per lane is a whole block's codes, and a block is whole 128-byte lines: with the scales
+// right behind each block, the lines that two blocks shared came from memory twice (7% more traffic at
+// groups of 128). Groups past K and rows past N have scale 0.
 #pragma once
 
 #include "ember_common.h"
@@ -100,7 +101,7 @@ __device__ __forceinline__ typename Mfma16<T>::v8 w4_values(uint32_t w) {
 constexpr int kW4Block = 128;  // k per block
 
 __host__ __device__ inline int w4_gpb(int64_t group) { return group >= kW4Block ? 1 : static_cast<int>(kW4Block / group); }
-__host__ __device__ inline int64_t w4_block_bytes(int gpb) { return 1024 + 64 * gpb; }
+__host__ __device__ inline int64_t w4_slab_bytes(int64_t nb, int gpb) { return nb * 1024 + (nb * 64 * gpb + 127) / 128 * 128; }
 
 // One block of R slabs, as loaded.
 template <int R, int GPB>
@@ -108,22 +109,22 @@ struct W4Block {
   u32x4 w[R];
   uint32_t m[R][GPB];
 
-  // slab: the slab's blocks. Buffer loads: the address is the resource, a scalar and one lane offset, so
+  // slab: the slab's bytes. Buffer loads: the address is the resource, a scalar and one lane offset, so
   // that no vector arithmetic goes into it.
-  __device__ __forceinline__ void load(int r, BufferRsrc slab, int block, int lane) {
-    const int at = block * (1024 + 64 * GPB);
-    w[r] = __builtin_amdgcn_raw_buffer_load_b128(slab, lane * 16, at, kPolicyNt);
+  __device__ __forceinline__ void load(int r, BufferRsrc slab, int block, int nb, int lane) {
+    w[r] = __builtin_amdgcn_raw_buffer_load_b128(slab, lane * 16, block * 1024, kPolicyNt);
+    const int at = nb * 1024 + block * (64 * GPB);
     const int mo = (lane & 15) * (4 * GPB);
     if constexpr (GPB == 4) {
-      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(slab, mo, at + 1024, 0);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(slab, mo, at, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) m[r][i] = v[i];
     } else if constexpr (GPB == 2) {
-      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(slab, mo, at + 1024, 0);
+      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(slab, mo, at, 0);
       m[r][0] = v[0];
       m[r][1] = v[1];
     } else {
-      m[r][0] = __builtin_amdgcn_raw_buffer_load_b32(slab, mo, at + 1024, 0);
+      m[r][0] = __builtin_amdgcn_raw_buffer_load_b32(slab, mo, at, 0);
     }
   }
 

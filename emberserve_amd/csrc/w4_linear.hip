@@ -53,7 +53,7 @@ k_w4_linear(W4Args a) {
 #pragma unroll
   for (int i = 0; i < NT * XI; ++i)
     off[i] = min(4 * i + (lane >> 4), rows - 1) * static_cast<int>(a.xs) * 2 + 16 * (lane & 15);
-  const int64_t slab_bytes = a.nb * w4_block_bytes(GPB);
+  const int64_t slab_bytes = w4_slab_bytes(a.nb, GPB);
   BufferRsrc base[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -74,7 +74,7 @@ k_w4_linear(W4Args a) {
       [&](Stage& g, int j) {
         const int b = min(wave + j * wk, a.nb - 1);
 #pragma unroll
-        for (int r = 0; r < R; ++r) g.w.load(r, base[r], b, lane);
+        for (int r = 0; r < R; ++r) g.w.load(r, base[r], b, a.nb, lane);
         g.x.load(xr, off, b, a.K, lane);
       },
       [&](const Stage& g, int) {
@@ -230,26 +230,24 @@ struct W4PackArgs {
   int64_t pieces;  // 16-byte pieces in all
 };
 
-// One 16-byte piece of the packed array a thread: lane `lane`'s codes of a block, or four scales.
+// One 16-byte piece of the packed array a thread: lane `lane`'s codes of a block, or four words of scales.
 __global__ void __launch_bounds__(256) k_w4_pack(W4PackArgs a) {
-  const int per = 64 + 4 * a.gpb;  // pieces of a block
+  const int64_t per = w4_slab_bytes(a.nb, a.gpb) / 16;  // pieces of a slab
   const int slabs = (a.rows + 15) / 16 * a.parts;
   for (int64_t t = int64_t(blockIdx.x) * 256 + threadIdx.x; t < a.pieces; t += int64_t(gridDim.x) * 256) {
-    int64_t q = t / per;
-    const int piece = static_cast<int>(t - q * per);
-    const int b = static_cast<int>(q % a.nb);
-    q /= a.nb;
-    const int s = static_cast<int>(q % slabs);
-    const int64_t e = q / slabs;
-    const int row0 = s / a.parts * 16;             // first row within the part
+    const int64_t sl = t / per;
+    const int piece = static_cast<int>(t - sl * per);
+    const int64_t e = sl / slabs;
+    const int s = static_cast<int>(sl - e * slabs);
+    const int row0 = s / a.parts * 16;  // first row within the part
     const int64_t part = int64_t(s % a.parts) * a.rows;
     u32x4 v = {0, 0, 0, 0};
-    if (piece < 64) {
-      const int row = row0 + (piece & 15);
+    if (piece < 64 * a.nb) {
+      const int lane = piece & 63, row = row0 + (lane & 15);
       if (row < a.rows) {
         const uint8_t* src = a.codes + e * a.ces + (part + row) * a.crs;
         for (int f = 0; f < 4; ++f) {
-          const int k0 = kW4Block * b + 32 * f + 8 * (piece >> 4);
+          const int k0 = kW4Block * (piece >> 6) + 32 * f + 8 * (lane >> 4);
           if (k0 >= a.k) continue;
           uint32_t w = 0;
           for (int i = 0; i < 4; ++i) {  // byte i: codes 2 i (low nibble) and 2 i + 1
@@ -261,15 +259,15 @@ __global__ void __launch_bounds__(256) k_w4_pack(W4PackArgs a) {
       }
     } else {
       for (int i = 0; i < 4; ++i) {
-        const int word = (piece - 64) * 4 + i;  // [row][gpb]
-        const int row = row0 + word / a.gpb;
-        const int k0 = kW4Block * b + word % a.gpb * (kW4Block / a.gpb);
+        const int word = (piece - 64 * a.nb) * 4 + i;  // [block][row][gpb]
+        const int row = row0 + word / a.gpb % 16;
+        const int k0 = kW4Block * (word / (16 * a.gpb)) + word % a.gpb * (kW4Block / a.gpb);
         if (row >= a.rows || k0 >= a.k) continue;
-        const int g = k0 / a.group;
-        const int64_t at = e * a.ses + (part + row) * a.srs + g;
+        const int64_t at = e * a.ses + (part + row) * a.srs + k0 / a.group;
         const float sc = a.scale_dtype == EMBER_F16 ? to_f32(static_cast<const _Float16*>(a.scales)[at])
                                                     : to_f32(static_cast<const __bf16*>(a.scales)[at]);
-        const uint32_t z = a.zeros != nullptr ? a.zeros[e * a.zes + (part + row) * a.zrs + g] & 15u : 8u;
+        const uint32_t z =
+            a.zeros != nullptr ? a.zeros[e * a.zes + (part + row) * a.zrs + k0 / a.group] & 15u : 8u;
         v[i] = (__builtin_bit_cast(uint32_t, sc) & ~15u) | z;
       }
     }
@@ -286,7 +284,7 @@ extern "C" {
 
 int64_t ember_w4_packed_bytes(int64_t rows, int64_t k, int64_t group, int gate_up) {
   if (!sizes_ok(rows, k, group)) return -1;
-  return cdiv(rows, 16) * (gate_up ? 2 : 1) * cdiv(k, kW4Block) * w4_block_bytes(w4_gpb(group));
+  return cdiv(rows, 16) * (gate_up ? 2 : 1) * w4_slab_bytes(cdiv(k, kW4Block), w4_gpb(group));
 }
 
 int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t code_row_stride, const void* scales,

@@ -83,14 +83,14 @@ class PackedW4:
         library GEMM at prefill sizes."""
         if self.parts is not None:
             return dequantize_w4(*self.parts, dtype=dtype)
-        gpb, nb = max(1, 128 // self.group), -(-self.k // 128)
-        blocks = self.packed.view(self.num_experts or 1, -1, nb, 1024 + 64 * gpb)
-        e, slabs = blocks.shape[:2]
-        words = blocks[..., :1024].contiguous().view(torch.int32).view(e, slabs, nb, 4, 16, 4)
+        gpb, nb, e = max(1, 128 // self.group), -(-self.k // 128), self.num_experts or 1
+        flat = self.packed.view(e, -1, 1024 * nb + -(-64 * gpb * nb // 128) * 128)
+        slabs = flat.shape[1]
+        words = flat[..., :1024 * nb].contiguous().view(torch.int32).view(e, slabs, nb, 4, 16, 4)
         q = torch.stack([(words >> (4 * (j // 2) + 16 * (j % 2))) & 15 for j in range(8)], dim=-1)
         q = q.permute(0, 1, 4, 2, 5, 3, 6).reshape(e, slabs, 16, nb * gpb, 128 // gpb)
-        meta = blocks[..., 1024:].contiguous().view(torch.int32).view(e, slabs, nb, 16, gpb).transpose(2, 3)
-        meta = meta.reshape(e, slabs, 16, nb * gpb, 1)
+        meta = flat[..., 1024 * nb:1024 * nb + 64 * gpb * nb].contiguous().view(torch.int32)
+        meta = meta.view(e, slabs, nb, 16, gpb).transpose(2, 3).reshape(e, slabs, 16, nb * gpb, 1)
         w = (q - (meta & 15)).float() * (meta & -16).view(torch.float32)
         halves = 2 if self.gate_up else 1
         w = w.reshape(e, slabs // halves, halves, 16, -1).transpose(1, 2).reshape(e, halves, -1, nb * 128)

@@ -622,8 +622,8 @@ int ember_moe_align(const void* topk_ids, int id_bytes, int64_t num_valid, int64
  * multiple of 128, and divides k. */
 
 /* Bytes of one expert's (or the only) packed weight, -1 for invalid arguments: slabs of 16 rows,
- * each ceil(k / 128) blocks of 1024 + 64 gpb bytes, gpb = 128 / group groups a block (1 from 128
- * on). gate_up: rows is one half's; gate and up slabs alternate. */
+ * each nb = ceil(k / 128) blocks of 1024 bytes and 64 gpb nb bytes of scales rounded up to 128, gpb =
+ * 128 / group groups a block (1 from 128 on). gate_up: rows is one half's; gate and up slabs alternate. */
 int64_t ember_w4_packed_bytes(int64_t rows, int64_t k, int64_t group, int gate_up);
 
 /* Packs codes [num_experts, rows, k / 2] (two to a byte, the even k in the low nibble), scales
@@ -633,7 +633,7 @@ int64_t ember_w4_packed_bytes(int64_t rows, int64_t k, int64_t group, int gate_u
  * num_experts * ember_w4_packed_bytes bytes, 16-byte aligned:
  *   block[lane][f]: the codes of row lane % 16 of the slab at k = 128 b + 32 f + 8 (lane / 16) + j,
  *                   j < 8, at bits 4 (j / 2) + 16 (j % 2)                (lane < 64, f < 4)
- *   then [row][gpb] words: the scale as fp32 bits, with its zero point in the low four bits. */
+ *   scales[block][row][gpb]: words, the scale as fp32 bits with its zero point in the low four. */
 int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t code_row_stride, const void* scales,
                          int64_t scale_expert_stride, int64_t scale_row_stride, int scale_dtype, const void* zeros,
                          int64_t zero_expert_stride, int64_t zero_row_stride, int64_t num_experts, int64_t rows,

@@ -171,7 +171,8 @@ def test_abi_argument_checks():
     lib = _lib.load()
     p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4100)  # never dereferenced: the calls are refused first
     size = lib.ember_w4_packed_bytes
-    assert size(16, 128, 128, 0) == 1088 and size(17, 129 + 31, 32, 0) == 2 * 2 * 1280 and size(16, 128, 64, 1) == 2304
+    assert size(16, 128, 128, 0) == 1024 + 128 and size(17, 129 + 31, 32, 0) == 2 * (2 * 1024 + 512)
+    assert size(16, 640, 64, 1) == 2 * (5 * 1024 + 640)
     for bad in ((0, 128, 128, 0), (16, 0, 128, 0), (16, 128, 96, 0), (16, 100, 32, 0), (16, 128, 256, 0),
                 (16, 128, 0, 0), (16, 128, -64, 0), (1 << 28, 128, 128, 0), (16, 1 << 25, 128, 0)):
         assert size(*bad) == -1
