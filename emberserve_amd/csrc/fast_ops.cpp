@@ -45,13 +45,15 @@ struct Entry {
 };
 enum {
   kRmsnorm, kAddRmsnorm, kRope, kSilu, kEmbedding, kQkNormRope, kMlaLatentRope, kRopeKvCache, kMlaLatentRopeCache,
-  kPagedDecode, kMlaDecode, kStatusString, kEntries
+  kPagedDecode, kMlaDecode, kW4Linear, kW4GateUp, kMoeLayer, kMoeLayerW4, kStatusString, kEntries
 };
 Entry g_entry[kEntries] = {
     {"ember_rmsnorm", nullptr}, {"ember_fused_add_rmsnorm", nullptr}, {"ember_rope", nullptr},
     {"ember_silu_and_mul", nullptr}, {"ember_embedding", nullptr}, {"ember_qk_norm_rope", nullptr},
     {"ember_mla_latent_rope", nullptr}, {"ember_rope_kv_cache", nullptr}, {"ember_mla_latent_rope_cache", nullptr},
-    {"ember_paged_decode_shared", nullptr}, {"ember_mla_decode", nullptr}, {"ember_status_string", nullptr}};
+    {"ember_paged_decode_shared", nullptr}, {"ember_mla_decode", nullptr},
+    {"ember_w4_linear", nullptr}, {"ember_w4_gate_up_silu", nullptr}, {"ember_moe_layer", nullptr},
+    {"ember_moe_layer_w4", nullptr}, {"ember_status_string", nullptr}};
 bool g_bound = false;
 
 #define ENTRY(i, f) reinterpret_cast<decltype(&f)>(g_entry[i].fn)
@@ -577,11 +579,100 @@ PyObject* mla_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The integers of a tuple of N. False (no error set) for anything else.
+template <size_t N>
+bool as_ints(PyObject* o, int64_t (&v)[N]) {
+  if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != static_cast<Py_ssize_t>(N)) return false;
+  for (size_t i = 0; i < N; ++i) {
+    v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, static_cast<Py_ssize_t>(i)));
+    if (v[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  return true;
+}
+
+// (x, packed, bias or None, (rows, k, group, gate_up)) -> out. The tuple is the packed weight's own.
+PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) Py_RETURN_NONE;
+  Call c;
+  const at::Tensor* x = c.tensor(a[0]);
+  const at::Tensor* w = c.tensor(a[1]);
+  const at::Tensor* bias = a[2] != Py_None ? c.tensor(a[2]) : nullptr;
+  int64_t shape[4];
+  if (!c.ok || !as_ints(a[3], shape)) Py_RETURN_NONE;
+  const int64_t rows = shape[0], k = shape[1], group = shape[2];
+  const Rows r(*x);
+  const int tag = dtype_tag(*x);
+  if (!r.ok || r.width != k || (tag != EMBER_F16 && tag != EMBER_BF16) ||
+      (bias != nullptr && (bias->dim() != 1 || bias->size(0) != rows || bias->scalar_type() != x->scalar_type() ||
+                           !bias->is_contiguous())))
+    Py_RETURN_NONE;
+  c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
+  sizes.back() = rows;
+  at::Tensor out = at::empty(sizes, x->options());
+  void* s = c.stream();
+  const int entry = shape[3] != 0 ? kW4GateUp : kW4Linear;
+  const int st = launch([&] {
+    return entry == kW4GateUp
+               ? ENTRY(kW4GateUp, ember_w4_gate_up_silu)(x->data_ptr(), r.stride, w->data_ptr(), group, tag, r.rows, k,
+                                                         rows, out.data_ptr(), rows, s)
+               : ENTRY(kW4Linear, ember_w4_linear)(x->data_ptr(), r.stride, w->data_ptr(), group, tag, r.rows, k, rows,
+                                                   bias != nullptr ? bias->data_ptr() : nullptr, out.data_ptr(), rows,
+                                                   s);
+  });
+  if (!answered(st, entry)) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, topk_ids, topk_weights, gate_up, down, (experts, hidden, inter, gate_up group, down group), plan) -> out,
+// over packed weights that fit the tuple (groups 0: 16 bits of x's dtype).
+PyObject* fused_moe(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  Call c;
+  const at::Tensor *x = c.tensor(a[0]), *ids = c.tensor(a[1]), *wt = c.tensor(a[2]), *w1 = c.tensor(a[3]),
+                   *w2 = c.tensor(a[4]);
+  int64_t shape[5];
+  if (!c.ok || !as_ints(a[5], shape)) Py_RETURN_NONE;
+  const int64_t e = shape[0], h = shape[1], i = shape[2], g1 = shape[3], g2 = shape[4];
+  const int tag = dtype_tag(*x), wtag = dtype_tag(*wt);
+  if (x->dim() != 2 || x->numel() == 0 || x->size(1) != h || x->stride(1) != 1 || (tag != EMBER_F16 && tag != EMBER_BF16) ||
+      ids->dim() != 2 || ids->size(0) != x->size(0) || ids->numel() == 0 || !ids->is_contiguous() ||
+      (ids->scalar_type() != at::kLong && ids->scalar_type() != at::kInt) || wt->sizes() != ids->sizes() ||
+      !wt->is_contiguous() || wtag < 0 || (g1 == 0 && (w1->scalar_type() != x->scalar_type() || w2->scalar_type() != x->scalar_type())))
+    Py_RETURN_NONE;
+  const int64_t t = x->size(0), k = ids->size(1);
+  const int id_bytes = ids->scalar_type() == at::kLong ? 8 : 4;
+  Plan p;
+  if (!p.resolve(a[6], {t, k, e, h, i}, a[0])) return nullptr;
+  if (p.ws == nullptr) Py_RETURN_NONE;  // sizes that the wrapper refuses
+  at::Tensor out = at::empty({t, h}, x->options());
+  void* s = c.stream();
+  const int entry = g1 != 0 ? kMoeLayerW4 : kMoeLayer;
+  const int st = launch([&] {
+    return entry == kMoeLayerW4
+               ? ENTRY(kMoeLayerW4, ember_moe_layer_w4)(x->data_ptr(), x->stride(0), ids->data_ptr(), id_bytes,
+                                                        wt->data_ptr(), wtag, t, k, w1->data_ptr(), g1, w2->data_ptr(),
+                                                        g2, tag, e, h, i, p.ws, p.ws_bytes, out.data_ptr(), h, s)
+               : ENTRY(kMoeLayer, ember_moe_layer)(x->data_ptr(), x->stride(0), ids->data_ptr(), id_bytes,
+                                                   wt->data_ptr(), wtag, t, k, w1->data_ptr(), 0, 0, w2->data_ptr(), 0,
+                                                   0, tag, e, h, i, p.ws, p.ws_bytes, out.data_ptr(), h, s);
+  });
+  if (!answered(st, entry)) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     {"bind", bind, METH_O, nullptr}, {"silu_and_mul", silu_and_mul, METH_O, nullptr},
     FAST(rmsnorm), FAST(add_rmsnorm), FAST(embedding), FAST(rope), FAST(qk_norm_rope), FAST(rope_kv_cache),
     FAST(mla_latent_rope), FAST(mla_latent_rope_cache), FAST(paged_decode), FAST(mla_decode),
+    FAST(w4_linear), FAST(fused_moe),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -453,6 +453,7 @@ def fused_moe_gate_up(x: Tensor, topk_ids: Tensor, w_gate_up: Tensor, *, num_spl
 LAYER_MAX_TOKENS = 64
 LAYER_MAX_ASSIGNMENTS = 512
 LAYER_MAX_EXPERTS = 1024
+LAYER_MAX_HIDDEN_W4 = 16384  # over 4-bit experts: four tokens' rows in LDS
 
 # Activations, group lists, split partials and arrival counters of ember_moe_layer: two launches share
 # them, so one buffer per (thread, device, stream).
@@ -534,6 +535,29 @@ def _layer_weight(what: str, w: Tensor | None, packed, gate_up: bool):
     return w, ((e, k, n // 2) if gate_up else (e, n, k)), w.dtype, w.device
 
 
+def _layer_plan(n: int, k: int, E: int, H: int, I: int, x: Tensor) -> tuple[int, Tensor | None]:
+    """(bytes of counters, workspace) of a call; (0, None) for sizes that the layer does not take."""
+    counters = c_int64(0)
+    need = _lib.load().ember_moe_layer_workspace_bytes(n, k, E, H, I, byref(counters))
+    if need < 0:
+        return 0, None
+    return counters.value, _LAYER_SCRATCH.get(need - counters.value, counters.value, x.device)
+
+
+def _layer_packed(packed, packed_down) -> tuple[int, int, int, int, int] | None:
+    """(E, H, I, gate_up group, down group) of two packed weights of one layer, for the native host path."""
+    if type(packed) is PackedW4 and type(packed_down) is PackedW4:
+        if packed.gate_up and not packed_down.gate_up and packed.packed is not None and packed_down.packed is not None \
+                and packed.num_experts is not None and (packed.num_experts, packed.k, packed.rows) == \
+                (packed_down.num_experts, packed_down.rows, packed_down.k):
+            return packed.num_experts, packed.k, packed.rows, packed.group, packed_down.group
+    elif type(packed) is PackedExperts and type(packed_down) is PackedDown:
+        if (packed.num_experts, packed.hidden, packed.inter) == (packed_down.num_experts, packed_down.hidden,
+                                                                 packed_down.inter):
+            return packed.num_experts, packed.hidden, packed.inter, 0, 0
+    return None
+
+
 def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor | None, w_down: Tensor | None, *,
               packed: PackedExperts | PackedW4 | None = None, packed_down: PackedDown | PackedW4 | None = None) -> Tensor:
     """The routed experts' layer of fused_moe_forward (moe_triton.py:332-345) for a decode step:
@@ -547,7 +571,12 @@ def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tens
     be 4-bit (`w4.pack_w4_gate_up` and `w4.pack_w4` of [E, ...] codes). The activations are rounded
     once, to x's dtype, between the products; the sums are fp32. An id of -1 adds nothing; other ids
     outside [0, E) neither, and set the error word. H and I are multiples of 64 (4-bit: of 32 and of
-    their groups)."""
+    their groups, H at most LAYER_MAX_HIDDEN_W4)."""
+    shape = _layer_packed(packed, packed_down)
+    if shape is not None and not _lib.tracing():
+        got = _lib.fast.fused_moe(x, topk_ids, topk_weights, packed.packed, packed_down.packed, shape, _layer_plan)
+        if got is not None:  # an ordinary call, answered by the native host path
+            return got
     for name, t in (("x", x), ("topk_ids", topk_ids), ("topk_weights", topk_weights)):
         if t.dim() != 2:
             raise ValueError(f"fused_moe: {name} must have two dimensions, got {tuple(t.shape)}")
@@ -586,11 +615,9 @@ def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tens
     if n == 0:
         return out
     lib = _lib.load()
-    counters = c_int64(0)
-    need = lib.ember_moe_layer_workspace_bytes(n, k, E, H, I, byref(counters))
-    if need < 0:
+    counters, ws = _layer_plan(n, k, E, H, I, x)
+    if ws is None or (w4 and H > LAYER_MAX_HIDDEN_W4):
         raise ValueError(f"fused_moe: H {H} and I {I} not supported")
-    ws = _LAYER_SCRATCH.get(need - counters.value, counters.value, x.device)
     head = (x.data_ptr(), x.stride(0), ids.data_ptr(), ids.element_size(), weights.data_ptr(),
             _lib.dtype_tag(weights.dtype), n, k)
     tail = (_lib.dtype_tag(x.dtype), E, H, I, ws.data_ptr(), ws.numel() * 4, out.data_ptr(), out.stride(0))
@@ -603,7 +630,7 @@ def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tens
         _launch("ember_moe_layer", lib.ember_moe_layer, x.device, *head, *up, *down, *tail)
     if _check_indices():
         end = ws.numel() * 4
-        _LAYER_SCRATCH.verify_counters(ws, end - counters.value, end)
+        _LAYER_SCRATCH.verify_counters(ws, end - counters, end)
         if _lib.read_errors(clear=True) & _lib.ERR_EXPERT_ID:
             raise IndexError(f"emberserve_amd.fused_moe: expert id outside [0, {E})")
     return out

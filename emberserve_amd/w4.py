@@ -77,6 +77,8 @@ class PackedW4:
                  group: int, gate_up: bool, device: torch.device) -> None:
         self.packed, self.parts, self.num_experts = packed, parts, num_experts
         self.rows, self.k, self.group, self.gate_up, self.device = rows, k, group, gate_up, device
+        # what the native host path takes of a projection's weight (None: left to the wrappers)
+        self.projection = (rows, k, group, int(gate_up)) if packed is not None and num_experts is None else None
 
     def dequantize(self, dtype: torch.dtype) -> Tensor:
         """The weight [..., N, K] in `dtype`, from the packed form: for the eager forms and for a
@@ -191,6 +193,10 @@ def _rows(x: Tensor) -> Tensor:
 
 def linear_w4(x: Tensor, weight: PackedW4, bias: Tensor | None = None) -> Tensor:
     """round(x @ w.T + bias) [..., N] over a weight from `pack_w4`; bias [N] of x's dtype or None."""
+    if type(weight) is PackedW4 and weight.projection is not None and not weight.gate_up and not _lib.tracing():
+        got = _lib.fast.w4_linear(x, weight.packed, bias, weight.projection)
+        if got is not None:  # an ordinary call, answered by the native host path
+            return got
     _check("linear_w4", x, weight, False)
     if bias is not None and (bias.shape != (weight.rows,) or bias.dtype != x.dtype or bias.device != x.device):
         raise ValueError(f"linear_w4: a bias of {weight.rows} elements of {x.dtype} on {x.device} expected, got "
@@ -211,6 +217,10 @@ def linear_w4(x: Tensor, weight: PackedW4, bias: Tensor | None = None) -> Tensor
 def gate_up_silu_w4(x: Tensor, weight: PackedW4) -> Tensor:
     """round(silu(gate) * up) [..., I] over a weight from `pack_w4_gate_up`: `gate_up_silu` with 4-bit
     weights."""
+    if type(weight) is PackedW4 and weight.projection is not None and weight.gate_up and not _lib.tracing():
+        got = _lib.fast.w4_linear(x, weight.packed, None, weight.projection)
+        if got is not None:
+            return got
     _check("gate_up_silu_w4", x, weight, True)
     if not fused_enabled(x):
         return gate_up_silu_w4_torch(x, weight)

@@ -226,6 +226,52 @@ def test_two_streams():
     assert all(torch.equal(g, want) for g in got)
 
 
+def test_native_host_path_equals_the_wrapper(monkeypatch):
+    """The same bits with and without the extension over both kinds of packed weights; what neither takes is
+    refused either way."""
+    x = torch.randn(5, 128, generator=torch.Generator().manual_seed(23)).to(BF).to(DEV)
+    w1, w2 = (v.to(DEV) for v in _half(8, 128, 64, BF, seed=24))
+    ids, weights = (v.to(DEV) for v in _routing(5, 2, 8, seed=25))
+    q1, q2 = _w4_experts(8, 128, 64, 32, True, BF, seed=26)
+    packs = [(moe.pack_moe_gate_up_weight(w1), moe.pack_moe_down_weight(w2)),
+             (w4.pack_w4_gate_up(*_dev(q1)), w4.pack_w4(*_dev(q2)))]
+
+    def run(p, x=x, ids=ids, weights=weights):
+        return moe.fused_moe(x, ids, weights, None, None, packed=p[0], packed_down=p[1])
+
+    def all_runs():
+        return [run(p, **c) for p in packs for c in (
+            {}, dict(ids=ids.int()), dict(weights=weights.to(BF)), dict(ids=ids.T.contiguous().T), dict(x=x[:1], ids=ids[:1], weights=weights[:1]),
+            dict(x=torch.cat([x, x], 1)[:, 4:132].clone()[:, :128]))]
+
+    got = all_runs()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "fast", _lib._Fast())
+        assert all(torch.equal(g, w) for g, w in zip(got, all_runs()))
+    for p in packs:
+        with pytest.raises(ValueError):
+            run(p, x=x.repeat(13, 1), ids=ids.repeat(13, 1), weights=weights.repeat(13, 1))  # 65 tokens
+        with pytest.raises(ValueError):
+            run(p, ids=ids[:4])
+        with pytest.raises(TypeError):
+            run(p, x=x.float())
+    with pytest.raises((TypeError, ValueError)):
+        run((packs[0][0], packs[1][1]))
+    with pytest.raises(TypeError):
+        run(packs[0], x=x.half())
+
+
+def test_check_indices_reads_the_error_word(monkeypatch):
+    monkeypatch.setenv("EMBERSERVE_CHECK_INDICES", "1")
+    x = torch.randn(3, 128, generator=torch.Generator().manual_seed(27)).to(BF).to(DEV)
+    w1, w2 = (v.to(DEV) for v in _half(4, 128, 64, BF, seed=28))
+    ids, weights = (v.to(DEV) for v in _routing(3, 2, 4, seed=29))
+    moe.fused_moe(x, ids, weights, w1, w2)
+    ids[1, 1] = 4
+    with pytest.raises(IndexError):
+        moe.fused_moe(x, ids, weights, w1, w2)
+
+
 def test_decode_step_of_w4_model(monkeypatch):
     """A step as a model runs it: qkv (bias), o, router, 4-bit experts and head, eager against fused."""
     h, i, experts = 256, 128, 8

@@ -178,5 +178,35 @@ def test_eager_form_of_a_gpu_weight(monkeypatch):
     check(w4.linear_w4(x.to(DEV), packed), want, bound + 300 * 2.0 ** -24 * (x.double().abs() @ w.abs().T))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_native_host_path_equals_the_wrappers(dtype, monkeypatch):
+    """The same bits, shapes and refusals with and without the extension, for calls it answers and calls
+    it leaves alone."""
+    parts, gu = _weight(40, 256, 64, True, dtype, seed=17), _weight(96, 256, 32, False, dtype, seed=18)
+    packed, packed_gu = w4.pack_w4(*_dev(parts)), w4.pack_w4_gate_up(*_dev(gu))
+    x = _x(6, 256, dtype, seed=19).to(DEV)
+    bias = torch.randn(80, generator=torch.Generator().manual_seed(20)).to(dtype).to(DEV)
+    wide = torch.zeros(6, 600, dtype=dtype, device=DEV)
+    wide[:, 8:264] = x
+    calls = [lambda: w4.linear_w4(x, packed), lambda: w4.linear_w4(x, packed, bias[:40]),
+             lambda: w4.linear_w4(x, packed, bias[::2]), lambda: w4.linear_w4(wide[:, 8:264], packed),
+             lambda: w4.linear_w4(wide[:, 9:265], packed), lambda: w4.linear_w4(x.view(2, 3, 256), packed),
+             lambda: w4.linear_w4(x[0], packed), lambda: w4.linear_w4(x[:0], packed),
+             lambda: w4.gate_up_silu_w4(x, packed_gu), lambda: w4.gate_up_silu_w4(x.view(3, 2, 256), packed_gu)]
+    got = [c() for c in calls]
+    monkeypatch.setattr(_lib, "fast", _lib._Fast())
+    for g, c in zip(got, calls):
+        want = c()
+        assert g.shape == want.shape and g.dtype == want.dtype and torch.equal(g, want)
+    monkeypatch.undo()
+    for bad in (lambda: w4.linear_w4(x, packed_gu), lambda: w4.gate_up_silu_w4(x, packed),
+                lambda: w4.linear_w4(x[:, :128], packed), lambda: w4.linear_w4(x, packed, bias),
+                lambda: w4.linear_w4(x, packed, bias[:40].cpu())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        w4.linear_w4(x.float(), packed)
+
+
 def test_no_error_bits():
     assert _lib.read_errors(clear=True) == 0

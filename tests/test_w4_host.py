@@ -230,3 +230,14 @@ def test_bounds_have_teeth():
         with pytest.raises(AssertionError):
             check((x.double() @ codes64(*parts)[0].T).to(BF), want, bound)
     assert tiny_step(BF) > 0
+
+
+def test_native_host_path_declines_other_calls():
+    """CPU tensors, wrong argument counts and anything but the weight's own tuple are the wrappers'."""
+    _lib.load()
+    x, b = torch.zeros(2, 128, dtype=BF), torch.zeros(16, 80, dtype=torch.uint8)
+    ids, wt = torch.zeros(2, 1, dtype=torch.int64), torch.ones(2, 1)
+    fast = _lib.fast
+    assert fast.w4_linear(x, b, None, (16, 128, 128, 0)) is None and fast.w4_linear(x) is None
+    assert fast.w4_linear(x, b, None, (16, 128)) is None and fast.w4_linear(x, b, "b", None) is None
+    assert fast.fused_moe(x, ids, wt, b, b, (1, 128, 64, 128, 64), None) is None and fast.fused_moe() is None
