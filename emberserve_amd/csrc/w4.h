@@ -103,6 +103,15 @@ constexpr int kW4Block = 128;  // k per block
 __host__ __device__ inline int w4_gpb(int64_t group) { return group >= kW4Block ? 1 : static_cast<int>(kW4Block / group); }
 __host__ __device__ inline int64_t w4_slab_bytes(int64_t nb, int gpb) { return nb * 1024 + (nb * 64 * gpb + 127) / 128 * 128; }
 
+// A workgroup barrier that waits for this wave's LDS accesses but not for its global loads (__syncthreads()
+// would drain the loads in flight). The asm keeps memory accesses from moving across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // One block of R slabs, as loaded.
 template <int R, int GPB>
 struct W4Block {
@@ -138,40 +147,62 @@ struct W4Block {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < GPB; ++g) {
-      V8 xv[NT][FG];
-      f32x4 xs[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        xs[nt] = zero;
-#pragma unroll
-        for (int f = 0; f < FG; ++f) {
-          xv[nt][f] = __builtin_bit_cast(V8, x(nt, g * FG + f));
-          xs[nt] = M::run(xv[nt][f], ones, xs[nt]);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        f32x4 part[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) part[nt] = zero;
-#pragma unroll
-        for (int f = 0; f < FG; ++f) {
-          const V8 wv = w4_values<T>(w[r][g * FG + f]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) part[nt] = M::run(xv[nt][f], wv, part[nt]);
-        }
+      f32x4 xs[NT], part[NT][R];
+      auto scale = [&](int r) {
         const float s = __builtin_bit_cast(float, m[r][g] & ~15u);
         const float z = -16.0f - static_cast<float>(m[r][g] & 15u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            acc[nt][r][i] = __builtin_fmaf(s, __builtin_fmaf(z, xs[nt][i], part[nt][i]), acc[nt][r][i]);
+            acc[nt][r][i] = __builtin_fmaf(s, __builtin_fmaf(z, xs[nt][i], part[nt][r][i]), acc[nt][r][i]);
 #if defined(__HIP_DEVICE_COMPILE__)
           // the sums are made here: put off, the parts of every group and slab are live at once, and spill
           asm volatile("" : "+v"(acc[nt][r]));
 #endif
         }
+      };
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        xs[nt] = zero;
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[nt][r] = zero;
+      }
+      if constexpr (NT <= 2) {  // the group's fragments at once, slab by slab
+        V8 xv[NT][FG];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int f = 0; f < FG; ++f) {
+            xv[nt][f] = __builtin_bit_cast(V8, x(nt, g * FG + f));
+            xs[nt] = M::run(xv[nt][f], ones, xs[nt]);
+          }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int f = 0; f < FG; ++f) {
+            const V8 wv = w4_values<T>(w[r][g * FG + f]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) part[nt][r] = M::run(xv[nt][f], wv, part[nt][r]);
+          }
+          scale(r);
+        }
+      } else {  // one step's fragments at once, for all slabs: fewer registers
+#pragma unroll
+        for (int f = 0; f < FG; ++f) {
+          V8 xv[NT], wv[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) wv[r] = w4_values<T>(w[r][g * FG + f]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            xv[nt] = __builtin_bit_cast(V8, x(nt, g * FG + f));
+            xs[nt] = M::run(xv[nt], ones, xs[nt]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) part[nt][r] = M::run(xv[nt], wv[r], part[nt][r]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) scale(r);
       }
     }
   }

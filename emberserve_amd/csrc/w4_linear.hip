@@ -25,6 +25,7 @@ struct W4Args {
   int groups;    // sets of R slabs
   int tiles;     // sets of 16 NT tokens
   int gate_up;
+  int side;      // k_w4_wide: waves side by side
 };
 
 constexpr int kXcds = 8;
@@ -123,15 +124,144 @@ k_w4_linear(W4Args a) {
   }
 }
 
+// Many slabs: G waves side by side, of R slabs each, share every block's tokens through LDS, in WK such
+// teams along k. A CU takes in about 10 bytes a clock whether they come from memory or L2 (6.4 TB/s over
+// all), so that the tokens count like weights: at 27 tokens and 4 slabs a workgroup they were twice the
+// weights' bytes. Each wave loads XS of a block's 4 NT pieces of 4 rows, D blocks ahead with its weights,
+// and puts them into LDS; one barrier a block, two buffers a team.
+constexpr int kWideWaves = 12;
+constexpr int kWideLds = 65536;
+
+template <typename T, int GPB, int NT, int XS, int D>
+__global__ void __launch_bounds__(kWideWaves * kWave)
+k_w4_wide(W4Args a) {
+  constexpr int R = 2;
+  extern __shared__ __attribute__((aligned(16))) u32x4 lds[];  // [team][2][256 NT], then the teams' sums
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int side = a.side, wk = (blockDim.x >> 6) / side;
+  const int team = wave / side, place = wave - team * side;
+  const int group = blockIdx.x * side + place;
+  const int slab0 = group * R, tok0 = 16 * NT * blockIdx.y;
+  const bool real = group < a.groups;  // the last workgroup's other waves only help with the tokens
+  const int rows = min(a.T - tok0, 16 * NT);
+  const BufferRsrc xr = buffer(static_cast<const T*>(a.x) + static_cast<int64_t>(tok0) * a.xs,
+                               static_cast<int>(((rows - 1) * a.xs + a.K) * 2));
+  int off[XS];
+#pragma unroll
+  for (int i = 0; i < XS; ++i)
+    off[i] = min(4 * (place + i * side) + (lane >> 4), rows - 1) * static_cast<int>(a.xs) * 2 + 16 * (lane & 15);
+  const int64_t slab_bytes = w4_slab_bytes(a.nb, GPB);
+  BufferRsrc base[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    base[r] = buffer(a.w + min(slab0 + r, a.slabs - 1) * slab_bytes, static_cast<int>(slab_bytes));
+
+  struct Stage {
+    W4Block<R, GPB> w;
+    u32x4 x[XS];
+  };
+  f32x4 acc[NT][R];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[nt][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  stream<Stage, D>(
+      0, (a.nb + wk - 1) / wk,  // the same for all waves: the barriers
+      [&](Stage& g, int j) {
+        const int b = min(team + j * wk, a.nb - 1);
+#pragma unroll
+        for (int r = 0; r < R; ++r) g.w.load(r, base[r], b, a.nb, lane);
+        const int past = nowhere(b * kW4Block + 8 * (lane & 15) >= a.K);
+#pragma unroll
+        for (int i = 0; i < XS; ++i) g.x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, off[i] | past, b * (2 * kW4Block), 0);
+      },
+      [&](const Stage& g, int j) {
+        u32x4* const x = lds + (team * 2 + (j & 1)) * (256 * NT);
+#pragma unroll
+        for (int i = 0; i < XS; ++i) {
+          const int r = 4 * (place + i * side) + (lane >> 4);
+          if (r < 16 * NT) x[16 * r + ((lane & 15) ^ (r & 15))] = g.x[i];
+        }
+        lds_barrier();
+        if (real && team + j * wk < a.nb)
+          g.w.template compute<T, NT>([&](int nt, int f) { return XBlock<NT, 4>::frag(x, nt, f, lane); }, acc);
+      });
+
+  // lane: column l % 16 of its slab, tokens 16 nt + 4 (l / 16) + i
+  f32x4* const red = reinterpret_cast<f32x4*>(lds) + place * (NT * R * kWave);
+  const int each = side * NT * R * kWave;
+  if (wk > 1) {
+    __syncthreads();
+    if (team > 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < R; ++r) red[(team - 1) * each + (nt * R + r) * kWave + lane] = acc[nt][r];
+    }
+    __syncthreads();
+  }
+  if (team > 0 || !real) return;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      for (int q = 0; q < wk - 1; ++q) acc[nt][r] += red[q * each + (nt * R + r) * kWave + lane];
+    auto put = [&](int slab, f32x4 v, f32x4 up) {
+      const int col = (a.gate_up ? slab >> 1 : slab) * 16 + (lane & 15);
+      if (slab >= a.slabs || col >= a.N) return;
+      const float bias = a.bias != nullptr ? to_f32(static_cast<const T*>(a.bias)[col]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 16 * nt + 4 * (lane >> 4) + i;
+        if (tok >= rows) continue;
+        const float y = a.gate_up ? silu_mul(v[i], up[i]) : v[i] + bias;
+        static_cast<T*>(a.out)[static_cast<int64_t>(tok0 + tok) * a.os + col] = from_f32<T>(y);
+      }
+    };
+    put(slab0, acc[nt][0], acc[nt][1]);
+    if (!a.gate_up) put(slab0 + 1, acc[nt][1], acc[nt][1]);
+  }
+}
+
+template <typename T, int GPB, int NT, int XS, int D>
+int wide_launch(W4Args a, int wk, hipStream_t stream) {
+  const size_t lds = std::max<size_t>(size_t(wk) * 2 * 4096 * NT, size_t(wk - 1) * a.side * NT * 2048);
+  const dim3 grid(static_cast<unsigned>(cdiv(a.groups, a.side)), static_cast<unsigned>(cdiv(a.T, 16 * NT)));
+  k_w4_wide<T, GPB, NT, XS, D><<<grid, a.side * wk * kWave, lds, stream>>>(a);
+  return launch_status();
+}
+
+// Waves side by side, for 9 tokens and more: the pairs of slabs that each CU gets, where that is 2 to 8 (one
+// round of workgroups). Measured (us, k_w4_linear | k_w4_wide): gate_up 768 pairs x 4096, 8 tokens 14.2 |
+// 15.2, 16: 16.6 | 15.9, 32: 21.3 | 19.8, 64 (two passes of 32 with 3 waves side by side) 28.5 | 37.2; 1184
+// pairs x 3584, 16: 23.0 | 19.4, 32: 28.6 | 24.8, 64: 42.2 | 35.2; the head's 4748 pairs x 4096, 16: 69.3 | 77.
+int wide_side(const W4Args& a) {
+  const int64_t cus = std::max(1, device_cu_count()), pairs = cdiv(a.slabs, 2), side = cdiv(pairs, cus);
+  if (a.T <= 8 || side > 8 || 4 * pairs < 7 * cus || (a.T > 32 && side < 4)) return 0;
+  return static_cast<int>(side);
+}
+
+template <typename T, int GPB>
+int wide_pick(W4Args a, hipStream_t stream) {
+  const bool most = a.side >= 4;
+  const int nt = a.T <= 16 ? 1 : (a.T <= 32 ? 2 : 4);
+  int wk = kWideWaves / a.side;
+  while (wk > 1 && (wk * 8192 * nt > kWideLds || (wk - 1) * a.side * nt * 2048 > kWideLds || 2 * wk > a.nb)) --wk;
+  if (nt == 1) return most ? wide_launch<T, GPB, 1, 1, 4>(a, wk, stream) : wide_launch<T, GPB, 1, 2, 4>(a, wk, stream);
+  if (nt == 2) return most ? wide_launch<T, GPB, 2, 2, 4>(a, wk, stream) : wide_launch<T, GPB, 2, 4, 3>(a, wk, stream);
+  return wide_launch<T, GPB, 4, 4, 2>(a, wk, stream);
+}
+
 template <typename T, int R, int GPB, int NT, int XI, int D, int MAXW>
 int w4_launch(W4Args a, hipStream_t stream) {
   const int64_t cus = std::max(1, device_cu_count());
   a.groups = static_cast<int>(cdiv(a.slabs, R));
   a.tiles = static_cast<int>(cdiv(a.T, 16 * NT));
   const int64_t grid = cdiv(a.groups, kXcds) * kXcds * a.tiles;
-  // Waves along k: 7 or more a CU, each with at least a block or two. Measured (us at 1 | 2 | 4 | 8 | 16):
-  // Qwen2.5-7B down, 2 tokens (224 slabs, 148 blocks) ... | 12.6 | 11.8 | 13.6; Qwen3-8B head, 16 tokens
-  // (2374 sets) 70.4 | 75.6 | 76.7.
+  // Waves along k: 7 or more a CU, each with at least a block or two. Measured (us): Qwen2.5-7B down, 2
+  // tokens (224 slabs, 148 blocks) 12.6 with 4, 11.8 with 8, 13.6 with 16; Qwen3-8B head, 16 tokens (2374
+  // sets of slabs) 70.4 with 1, 75.6 with 2.
   int wk = 1;
   while (wk < MAXW && grid * wk < 7 * cus && 2 * wk < a.nb) wk *= 2;
   const size_t lds = size_t(wk) * 16 * std::max(XBlock<NT, XI>::kPieces, 64 * R * NT);
@@ -161,10 +291,15 @@ int w4_slabs(const W4Args& a, int tokens) {
 // once for both (gate_up of Qwen2.5-7B, 27 tokens, 35.6 us with one tile a wave, 28.8 with two). Up to 4
 // and 8 tokens a block's tokens are one and two loads instead of four, and the ring is deeper.
 template <typename T, int GPB>
-int w4_pick(const W4Args& a, hipStream_t stream) {
+int w4_pick(W4Args a, hipStream_t stream) {
   if (a.T <= 4) {
     if (!a.gate_up) return w4_launch<T, 1, GPB, 1, 1, GPB == 4 ? 6 : 8, 16>(a, stream);
     return w4_launch<T, 2, GPB, 1, 1, GPB == 4 ? 3 : 4, 16>(a, stream);
+  }
+  if (const int side = wide_side(a); side != 0) {
+    a.groups = static_cast<int>(cdiv(a.slabs, 2));
+    a.side = side;
+    return wide_pick<T, GPB>(a, stream);
   }
   const int r = w4_slabs(a, a.T <= 16 ? 16 : 32);
   if (a.T <= 8) {
@@ -209,7 +344,7 @@ int w4_call(const void* x, int64_t xs, const void* packed, int64_t group, int dt
   if (!aligned16(x) || !aligned16(packed) || xs % 8 != 0) return EMBER_EALIGN;
   W4Args a{x, xs, static_cast<const uint8_t*>(packed), bias, out, os, static_cast<int>(tokens), static_cast<int>(k),
            static_cast<int>(rows), static_cast<int>(cdiv(rows, 16)) * (gate_up ? 2 : 1),
-           static_cast<int>(cdiv(k, kW4Block)), 0, 1, gate_up};
+           static_cast<int>(cdiv(k, kW4Block)), 0, 1, gate_up, 0};
   const int gpb = w4_gpb(group);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == EMBER_F16 ? w4_run<_Float16>(a, gpb, s) : w4_run<__bf16>(a, gpb, s);

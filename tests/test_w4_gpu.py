@@ -51,7 +51,9 @@ def test_pack_round_trip(n, k, group, gate_up):
     (1, 16, 32, 32, False), (1, 1, 64, 64, True), (3, 17, 96, 32, True), (16, 48, 896, 128, False),
     (17, 1152, 896, 64, True), (33, 100, 4864, 128, True), (64, 272, 1024, 32, False), (65, 33, 160, 32, True),
     (200, 64, 384, 128, False), (2, 3584, 2048, 512, True), (5, 40000, 256, 128, False), (31, 70001, 128, 64, True),
-    (50, 70000, 64, 32, False)])
+    (50, 70000, 64, 32, False),
+    (9, 14500, 160, 32, True), (32, 14340, 384, 128, False), (40, 33000, 96, 32, False), (64, 57000, 128, 64, True),
+    (90, 31000, 160, 32, True), (16, 65500, 128, 128, False)])
 def test_linear_matches_64_bits(dtype, t, n, k, group, zeros):
     print(f"linear_w4 {t}x{n}x{k} g{group} zeros={zeros} {dtype}", flush=True)
     parts, x = _weight(n, k, group, zeros, dtype, seed=t + n), _x(t, k, dtype, seed=k)
@@ -69,7 +71,9 @@ def test_linear_matches_64_bits(dtype, t, n, k, group, zeros):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("t,inter,k,group,zeros", [
     (1, 16, 32, 32, True), (2, 5, 128, 128, False), (16, 4864, 896, 128, True), (27, 77, 416, 32, True),
-    (64, 160, 512, 64, False), (70, 30, 256, 256, True), (9, 40000, 128, 64, False), (40, 33000, 64, 32, True)])
+    (64, 160, 512, 64, False), (70, 30, 256, 256, True), (9, 40000, 128, 64, False), (40, 33000, 64, 32, True),
+    (9, 7200, 160, 32, True), (17, 7205, 640, 128, False), (31, 12290, 384, 64, True), (33, 16400, 96, 32, False),
+    (64, 18944, 256, 128, True), (100, 16385, 128, 64, False), (12, 32760, 160, 32, False)])
 def test_gate_up_matches_64_bits(dtype, t, inter, k, group, zeros):
     print(f"gate_up_silu_w4 {t}x{inter}x{k} g{group} zeros={zeros} {dtype}", flush=True)
     parts, x = _weight(2 * inter, k, group, zeros, dtype, seed=t + inter), _x(t, k, dtype, seed=k)
