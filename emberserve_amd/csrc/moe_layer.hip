@@ -52,6 +52,7 @@ struct MlArgs {
   void* out;
   int64_t os;
   int tile;           // assignments of a group: 4, 8 or 16
+  int max_groups;     // groups that the assignments can form
   int slabs;          // column slabs (second kernel: slab sets) of the grid
   int per_wg, wk;     // 4 bits, first kernel: slabs of a workgroup, waves that share a slab's k
   int splits;         // of the second kernel's work
@@ -316,7 +317,7 @@ struct Down {
     sums = all + wave * a.N * kCols;
     wts = all + W * a.N * kCols;
     lists = reinterpret_cast<int16_t*>(wts + (a.A + 3) / 4 * 4);
-    experts = lists + G * kMlTile;
+    experts = lists + a.max_groups * kMlTile;  // all that there can be: their loads need not wait for G
     for (int i = lane; i < a.N * kCols; i += kWave) sums[i] = 0.f;
     for (int i = threadIdx.x; i < a.A; i += W * kWave) {
       float w;
@@ -325,9 +326,9 @@ struct Down {
       else w = to_f32(static_cast<const __bf16*>(a.weights)[i]);
       wts[i] = w;
     }
-    for (int i = threadIdx.x; i < G * kMlTile / 8; i += W * kWave)
+    for (int i = threadIdx.x; i < a.max_groups * kMlTile / 8; i += W * kWave)
       reinterpret_cast<u32x4*>(lists)[i] = reinterpret_cast<const u32x4*>(a.glist)[i];
-    for (int i = threadIdx.x; i < G; i += W * kWave) experts[i] = static_cast<int16_t>(a.gexpert[1 + i]);
+    for (int i = threadIdx.x; i < a.max_groups; i += W * kWave) experts[i] = static_cast<int16_t>(a.gexpert[1 + i]);
     __syncthreads();
   }
   // this wave's items, of n a group
@@ -535,13 +536,13 @@ bool ml_sizes_ok(int64_t N, int64_t top_k, int64_t E, int64_t H, int64_t I) {
 }
 
 size_t down_lds(const MlArgs& a, int waves, int cols) {
-  return 4 * (size_t(waves) * a.N * cols + a.A + 3) + 2 * size_t(max_groups(a.A, a.E, a.tile)) * (kMlTile + 1) + 16;
+  return 4 * (size_t(waves) * a.N * cols + a.A + 3) + 2 * size_t(a.max_groups) * (kMlTile + 1) + 16;
 }
 
 template <typename T>
 int ml_half(MlArgs a, hipStream_t s) {
   a.slabs = a.I / 16;
-  const int64_t grid = max_groups(a.A, a.E, a.tile) * a.slabs;
+  const int64_t grid = static_cast<int64_t>(a.max_groups) * a.slabs;
   k_moe_layer_up<T><<<dim3(static_cast<unsigned>(grid)), kUpWaves * kWave, 0, s>>>(a);
   if (const int st = launch_status(); st != EMBER_OK) return st;
   a.slabs = a.H / 16;
@@ -554,7 +555,7 @@ int ml_half(MlArgs a, hipStream_t s) {
 template <typename T, int GPB, int XI>
 int ml_up_w4(MlArgs a, hipStream_t s) {
   a.slabs = a.I / 16;
-  const int64_t groups = max_groups(a.A, a.E, a.tile), cus = std::max(1, device_cu_count());
+  const int64_t groups = a.max_groups, cus = std::max(1, device_cu_count());
   // Whole slabs a wave once they fill the chip twice over; until then the waves share a slab's k: four of
   // them, so that a token's workgroups are on the chip at once (Moonlight's 528: 8 waves each took two turns)
   const bool whole = groups * a.slabs >= 2 * kUpWavesW4 * cus;
@@ -650,6 +651,7 @@ int ml_call(const MlCall& c, const WeightView& w1, const WeightView& w2, int gpb
   a.os = c.os;
   a.packed_out = (reinterpret_cast<uintptr_t>(c.out) | (c.os * 2)) % 8 == 0;
   a.tile = group_tile(a.A, a.E, a.H, gpb1 > 0);
+  a.max_groups = static_cast<int>(max_groups(a.A, a.E, a.tile));
   a.err = err;
   hipStream_t s = static_cast<hipStream_t>(c.stream);
   return c.dtype == EMBER_F16 ? ml_run<_Float16>(a, gpb1, gpb2, s) : ml_run<__bf16>(a, gpb1, gpb2, s);
