@@ -26,7 +26,7 @@ from . import ops as _ops
 
 __all__ = ["rmsnorm", "fused_add_rmsnorm", "rope", "silu_and_mul", "embedding", "qk_norm_rope",
            "mla_latent_rope", "kv_cache_write", "latent_cache_write", "paged_attention_decode", "mla_decode",
-           "gate_up_silu", "moe_gate_up_silu"]
+           "gate_up_silu", "moe_gate_up_silu", "fused_moe", "linear_w4", "gate_up_silu_w4"]
 
 
 def _empty(shape, like: Tensor) -> Tensor:
@@ -135,6 +135,52 @@ def _fused_moe_gate_up(x: Tensor, topk_ids: Tensor, w_gate_up: Tensor) -> Tensor
 @_fused_moe_gate_up.register_fake
 def _(x, topk_ids, w_gate_up):
     return _empty((topk_ids.numel(), w_gate_up.shape[1] // 2), x)
+
+
+@custom_op("emberserve::fused_moe", mutates_args=())
+def _fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
+    from .moe import fused_moe as impl
+    return impl(x, topk_ids, topk_weights, w_gate_up, w_down)
+
+
+@_fused_moe.register_fake
+def _(x, topk_ids, topk_weights, w_gate_up, w_down):
+    return _empty(x.shape, x)
+
+
+# ---- projections over packed 4-bit weights (no counterpart in the reference) ---------------
+# A packed weight crosses the dispatcher as its bytes and its sizes: `PackedW4.packed`, rows, k, group.
+
+def _packed_w4(packed: Tensor, rows: int, k: int, group: int, gate_up: bool):
+    from . import _lib
+    from .w4 import PackedW4
+    need = _lib.load().ember_w4_packed_bytes(rows, k, group, int(gate_up))
+    if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.numel() != need:
+        raise ValueError(f"linear_w4: {need} contiguous bytes of a packed [{rows}, {k}] weight expected, got "
+                         f"{tuple(packed.shape)} {packed.dtype}")
+    return PackedW4(packed, None, None, rows, k, group, gate_up, packed.device)
+
+
+@custom_op("emberserve::linear_w4", mutates_args=())
+def _linear_w4(x: Tensor, packed: Tensor, bias: Tensor | None, rows: int, k: int, group: int) -> Tensor:
+    from .w4 import linear_w4 as impl
+    return impl(x, _packed_w4(packed, rows, k, group, False), bias)
+
+
+@_linear_w4.register_fake
+def _(x, packed, bias, rows, k, group):
+    return _empty(tuple(x.shape[:-1]) + (rows,), x)
+
+
+@custom_op("emberserve::gate_up_silu_w4", mutates_args=())
+def _gate_up_silu_w4(x: Tensor, packed: Tensor, inter: int, k: int, group: int) -> Tensor:
+    from .w4 import gate_up_silu_w4 as impl
+    return impl(x, _packed_w4(packed, inter, k, group, True))
+
+
+@_gate_up_silu_w4.register_fake
+def _(x, packed, inter, k, group):
+    return _empty(tuple(x.shape[:-1]) + (inter,), x)
 
 
 # ---- embedding (nn.Embedding in model/qwen2.py:172) ---------------------------------------
@@ -266,6 +312,20 @@ def moe_align(topk_ids: Tensor, num_experts: int, block_m: int = 16) -> tuple[Te
 
 def fused_moe_gate_up(x: Tensor, topk_ids: Tensor, w_gate_up: Tensor) -> Tensor:
     return torch.ops.emberserve.fused_moe_gate_up(x, topk_ids, w_gate_up)
+
+
+def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
+    return torch.ops.emberserve.fused_moe(x, topk_ids, topk_weights, w_gate_up, w_down)
+
+
+def linear_w4(x: Tensor, weight, bias: Tensor | None = None) -> Tensor:
+    """`w4.linear_w4` over a `PackedW4` on the GPU."""
+    return torch.ops.emberserve.linear_w4(x, weight.packed, bias, weight.rows, weight.k, weight.group)
+
+
+def gate_up_silu_w4(x: Tensor, weight) -> Tensor:
+    """`w4.gate_up_silu_w4` over a `PackedW4` on the GPU."""
+    return torch.ops.emberserve.gate_up_silu_w4(x, weight.packed, weight.rows, weight.k, weight.group)
 
 
 def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, eps: float, cos: Tensor,

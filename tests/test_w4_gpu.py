@@ -212,5 +212,21 @@ def test_native_host_path_equals_the_wrappers(dtype, monkeypatch):
         w4.linear_w4(x.float(), packed)
 
 
+def test_registered_ops():
+    """Schemas, fake kernels and results of torch.ops.emberserve's forms, and one traced by torch.compile."""
+    from emberserve_amd import torch_ops
+    parts, gu = _weight(48, 128, 64, True, BF, seed=21), _weight(64, 128, 32, False, BF, seed=22)
+    packed, packed_gu = w4.pack_w4(*_dev(parts)), w4.pack_w4_gate_up(*_dev(gu))
+    x = _x(3, 128, BF, seed=23).to(DEV)
+    torch.library.opcheck(torch.ops.emberserve.linear_w4, (x, packed.packed, None, 48, 128, 64))
+    torch.library.opcheck(torch.ops.emberserve.gate_up_silu_w4, (x, packed_gu.packed, 32, 128, 32))
+    assert torch.equal(torch_ops.linear_w4(x, packed), w4.linear_w4(x, packed))
+    assert torch.equal(torch_ops.gate_up_silu_w4(x, packed_gu), w4.gate_up_silu_w4(x, packed_gu))
+    with pytest.raises(ValueError):
+        torch.ops.emberserve.linear_w4(x, packed.packed[:, :1024].contiguous(), None, 48, 128, 64)
+    compiled = torch.compile(lambda v: torch_ops.linear_w4(v, packed) * 2, backend="aot_eager", fullgraph=True)
+    assert torch.equal(compiled(x), w4.linear_w4(x, packed) * 2)
+
+
 def test_no_error_bits():
     assert _lib.read_errors(clear=True) == 0

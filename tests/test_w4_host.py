@@ -241,3 +241,11 @@ def test_native_host_path_declines_other_calls():
     assert fast.w4_linear(x, b, None, (16, 128, 128, 0)) is None and fast.w4_linear(x) is None
     assert fast.w4_linear(x, b, None, (16, 128)) is None and fast.w4_linear(x, b, "b", None) is None
     assert fast.fused_moe(x, ids, wt, b, b, (1, 128, 64, 128, 64), None) is None and fast.fused_moe() is None
+
+
+def test_fused_moe_is_registered():
+    from emberserve_amd import torch_ops
+    x, w1, w2 = torch.randn(4, 64).to(BF), _w(128, 64, BF, 3), _w(64, 64, BF, 3)
+    ids, wt = torch.tensor([[0, 2], [1, 1], [2, 0], [-1, 1]]), torch.rand(4, 2)
+    torch.library.opcheck(torch.ops.emberserve.fused_moe, (x, ids, wt, w1, w2))
+    assert torch.equal(torch_ops.fused_moe(x, ids, wt, w1, w2), moe.fused_moe(x, ids, wt, w1, w2))
