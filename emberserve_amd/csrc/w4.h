@@ -168,7 +168,7 @@ struct W4Block {
 #pragma unroll
         for (int r = 0; r < R; ++r) part[nt][r] = zero;
       }
-      if constexpr (NT <= 2) {  // the group's fragments at once, slab by slab
+      if constexpr (R > 2) {  // slab by slab: fewer registers
         V8 xv[NT][FG];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -187,7 +187,7 @@ struct W4Block {
           }
           scale(r);
         }
-      } else {  // one step's fragments at once, for all slabs: fewer registers
+      } else {  // step by step: the chains of all slabs and tiles side by side (3% faster at one token)
 #pragma unroll
         for (int f = 0; f < FG; ++f) {
           V8 xv[NT], wv[R];
