@@ -90,13 +90,16 @@ class SharedScratch(_Verified):
 
     A call captured where no eager call has left a large enough workspace gets one that belongs to
     that capture: its memory is the graph's own, and the zero fill of its counters is recorded in
-    the graph, which therefore replays correctly whichever graphs ran before it."""
+    the graph, which therefore replays correctly whichever graphs ran before it. With `per_capture`
+    every capture gets one of its own, also where an eager call on its stream left a workspace: its
+    graphs then replay beside each other and beside eager calls."""
 
     MIN_PARTIAL = 1 << 20
     MIN_COUNTERS = 1 << 14
 
-    def __init__(self, what: str) -> None:
+    def __init__(self, what: str, per_capture: bool = False) -> None:
         self.what = what
+        self.per_capture = per_capture
         self._bufs: dict[tuple, _Buffer] = {}
         self._captured: dict[tuple, _Buffer] = {}
         self._outgrown: list[Tensor] = []
@@ -105,7 +108,7 @@ class SharedScratch(_Verified):
     def get(self, partial: int, counters: int, device: torch.device) -> Tensor:
         """A workspace for `partial` bytes of partials and `counters` bytes of counters."""
         key = (threading.get_ident(), device.index, _stream_key(device))
-        buf = self._bufs.get(key)
+        buf = None if self.per_capture and _capturing(device) else self._bufs.get(key)
         if buf is None or partial > buf.partial or counters > buf.counters:
             buf = self._grow(key, partial, counters, device)
         return buf.tensor
@@ -134,9 +137,13 @@ class SharedScratch(_Verified):
         return 4 * (sum(b.tensor.numel() for b in self._bufs.values()) + sum(t.numel() for t in self._outgrown))
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 def _capture_id(device: torch.device) -> int:
     """The id of the capture that the current stream takes part in, 0 outside one."""
-    if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+    if not _capturing(device):
         return 0
     got = c_uint64(0)
     _lib.check(_lib.load().ember_stream_capture_id(_stream_key(device), byref(got)), "ember_stream_capture_id")

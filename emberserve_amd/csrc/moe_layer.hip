@@ -2,20 +2,28 @@
 //   act[a, j] = round(silu(x[t] . W1[e, j]) * (x[t] . W1[e, I + j]))     a = t * top_k + c, e = ids[t, c]
 //   out[t, n] = round(sum_c weights[t, c] * (W2[e, n] . act[a]))
 // (fused_moe_forward, emberserve/model/moe_triton.py:332-345), over fp16/bf16 experts, unpacked or
-// packed, and over 4-bit experts. g, u and the routed sum stay in fp32; act is rounded once, to be an
-// MFMA operand.
+// packed, and over 4-bit experts (w4.h). g, u and the routed sum stay in fp32; act is rounded once, to be
+// an MFMA operand: half a step of the type on each of I terms, which at random signs adds as much to the
+// mean error of out as its own rounding does (bf16: 2.4e-3 of the rms, 1.7e-3 from the last rounding alone).
 //
 // What bounds it: the weights of the experts that the step's tokens reach, each read once. The
-// assignments of an expert form groups of 16 (an MFMA tile). Every workgroup of the first kernel finds
-// its group in the routing ids by itself, so there is no alignment launch: group u of the experts in
-// ascending order, with at most min(A, E) + A / 16 of them for A assignments. Its four waves share the
-// group's k for 16 gate and 16 up rows and meet in LDS.
+// assignments of an expert form groups, of up to 16 (an MFMA tile); 4-bit weights take groups of 4 or 8
+// where the mean is small. Every workgroup of the first kernel finds its group in the routing ids by
+// itself, so there is no alignment launch: up to 64 assignments, one a lane, by comparing lanes; else by
+// a count in LDS. Its waves share the group's k for 16 gate and 16 up rows and meet in LDS; over 4-bit
+// weights and enough groups they take 8 column slabs side by side instead, the group's tokens in LDS once.
 //
-// The second kernel's workgroups hold 16 output columns each for all groups (times a split of the work):
-// the waves cut the (group, k block) items of their columns into equal runs, whatever expert they belong
-// to, and add each group's finished tile, weighted, to their own fp32 sums [token][16] in LDS. The sums
-// of the waves, then of the splits (the last to arrive), are added in order, so that results do not
-// depend on which wave was first.
+// The second kernel's workgroups hold 16 (4 bits: 32) output columns each for all groups, times a split of
+// the work: the waves cut the (group, k block) items of their columns into equal runs, whatever expert
+// they belong to, and add each group's finished tile, weighted, to their own fp32 sums [token][column] in
+// LDS. The sums of the waves, then of the splits (by the last to arrive, in batches of 16-byte loads: one
+// load at a time took 20 us of 52 at 33 tokens), are added in order, so that results do not depend on
+// which wave was first.
+//
+// Measured (Moonlight, 64 experts top-6 of 2048 x 1408, us, first | second kernel): one token 16 | 11,
+// 9 tokens 62-68 | 36, 48 tokens 109 | 59 (1047 MB at 6.0 TB/s in all); 4 bits, one token 11 | 9, most of it
+// the chain of dependent loads (ids, weights; lists, weights, partials); 128 experts top-8 of 2048 x 768,
+// 4 bits, 33 tokens 45 | 29 (268 MB at 3.6 TB/s: the products' issue beside the stream).
 #include <algorithm>
 
 #include "w4.h"
@@ -29,6 +37,7 @@ constexpr int kMlMaxAssign = 512;
 constexpr int kMlMaxExperts = 1024;
 constexpr int64_t kMlMaxStride = 1 << 23;  // of x: 32-bit offsets over 64 rows
 constexpr int kMlMaxSplits = 16;
+constexpr int64_t kMlMaxSize = 1 << 18;    // of H and I: grids under 2^32 threads
 constexpr int kMlTokenLds = 128 << 10;      // a group's tokens, 4-bit weights
 constexpr int kMlMaxHiddenW4 = kMlTokenLds / 8;  // ... of four rows
 constexpr int kUpWaves = 4, kDownWaves = 8;      // 16-bit weights
@@ -532,7 +541,7 @@ MlLayout ml_layout(int64_t N, int64_t top_k, int64_t E, int64_t H, int64_t I) {
 
 bool ml_sizes_ok(int64_t N, int64_t top_k, int64_t E, int64_t H, int64_t I) {
   return N >= 0 && N <= kMlMaxTokens && top_k >= 1 && N * top_k <= kMlMaxAssign && top_k <= kMlMaxAssign && E >= 1 &&
-         E <= kMlMaxExperts && H >= 32 && I >= 32 && H % 32 == 0 && I % 32 == 0 && H <= (1 << 20) && I <= (1 << 20);
+         E <= kMlMaxExperts && H >= 32 && I >= 32 && H % 32 == 0 && I % 32 == 0 && H <= kMlMaxSize && I <= kMlMaxSize;
 }
 
 size_t down_lds(const MlArgs& a, int waves, int cols) {

@@ -456,8 +456,8 @@ LAYER_MAX_EXPERTS = 1024
 LAYER_MAX_HIDDEN_W4 = 16384  # over 4-bit experts: four tokens' rows in LDS
 
 # Activations, group lists, split partials and arrival counters of ember_moe_layer: two launches share
-# them, so one buffer per (thread, device, stream).
-_LAYER_SCRATCH = SharedScratch("fused_moe")
+# them, so one buffer per (thread, device, stream), and one per graph capture.
+_LAYER_SCRATCH = SharedScratch("fused_moe", per_capture=True)
 
 
 class PackedDown:
@@ -569,9 +569,9 @@ def fused_moe(x: Tensor, topk_ids: Tensor, topk_weights: Tensor, w_gate_up: Tens
     (`pack_moe_gate_up_weight`, the copy `fused_moe_gate_up` also reads) and `packed_down`
     (`pack_moe_down_weight`) are read instead where given, and the weight may then be None; both may
     be 4-bit (`w4.pack_w4_gate_up` and `w4.pack_w4` of [E, ...] codes). The activations are rounded
-    once, to x's dtype, between the products; the sums are fp32. An id of -1 adds nothing; other ids
-    outside [0, E) neither, and set the error word. H and I are multiples of 64 (4-bit: of 32 and of
-    their groups, H at most LAYER_MAX_HIDDEN_W4)."""
+    once, to x's dtype, between the products (in fp16, one past 65504 becomes infinite); the sums are
+    fp32. An id of -1 adds nothing; other ids outside [0, E) neither, and set the error word. H and I are
+    multiples of 64 (4-bit: of 32 and of their groups, H at most LAYER_MAX_HIDDEN_W4)."""
     shape = _layer_packed(packed, packed_down)
     if shape is not None and not _lib.tracing():
         got = _lib.fast.fused_moe(x, topk_ids, topk_weights, packed.packed, packed_down.packed, shape, _layer_plan)

@@ -210,6 +210,112 @@ def test_graph_replays_match_eager():
         assert torch.equal(outs[i % 2], moe.fused_moe(x, ids, weights, w1, w2)), i
 
 
+def test_two_graphs_of_one_stream_replay_at_once():
+    """Two graphs captured on a stream that eager calls used have workspaces of their own."""
+    w1, w2 = (v.to(DEV) for v in _half(16, 1024, 256, BF, seed=31))
+    ids, weights = (v.to(DEV) for v in _routing(8, 4, 16, seed=32))
+    xs = [torch.randn(8, 1024, generator=torch.Generator().manual_seed(33 + i)).to(BF).to(DEV) for i in range(3)]
+    want = [moe.fused_moe(x, ids, weights, w1, w2) for x in xs]
+    torch.cuda.synchronize()
+    one, graphs, outs = torch.cuda.Stream(), [], []
+    with torch.cuda.stream(one):
+        moe.fused_moe(xs[2], ids, weights, w1, w2)
+    for x in xs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=one):
+            outs.append([moe.fused_moe(x, ids, weights, w1, w2) for _ in range(4)])
+        graphs.append(g)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for g, s in zip(graphs, sides):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(one):
+            eager = moe.fused_moe(xs[2], ids, weights, w1, w2)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i]) and torch.equal(eager, want[2])
+
+
+@pytest.mark.parametrize("n,k,experts,h,i", [(33, 4, 8, 4096, 64), (20, 2, 4, 7168, 64), (2, 2, 2, 16384, 32)])
+def test_w4_long_rows(n, k, experts, h, i):
+    """Groups whose tokens take up to 128 KiB of LDS, eager and captured."""
+    x = torch.randn(n, h, generator=torch.Generator().manual_seed(n)).to(BF)
+    q1, q2 = _w4_experts(experts, h, i, 32, False, BF, seed=40)
+    ids, weights = _routing(n, k, experts, seed=41)
+    (w1, s1), (w2, s2) = codes64(*q1), codes64(*q2)
+    want, bound = _want(x, ids, weights, w1, w2, s1, s2, 32, 32)
+    packs = dict(packed=w4.pack_w4_gate_up(*_dev(q1)), packed_down=w4.pack_w4(*_dev(q2)))
+    args = [v.to(DEV) for v in (x, ids, weights)]
+    got = moe.fused_moe(*args, None, None, **packs)
+    check(got, want, bound)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = moe.fused_moe(*args, None, None, **packs)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, got)
+
+
+def test_w4_hidden_past_the_limit_is_refused():
+    q1, q2 = _w4_experts(1, 16416, 32, 32, False, BF, seed=42)
+    x, weights = torch.zeros(1, 16416, dtype=BF, device=DEV), torch.ones(1, 1, device=DEV)
+    ids = torch.zeros(1, 1, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError):
+        moe.fused_moe(x, ids, weights, None, None, packed=w4.pack_w4_gate_up(*_dev(q1)), packed_down=w4.pack_w4(*_dev(q2)))
+
+
+@pytest.mark.parametrize("w4_bits", [False, True])
+def test_more_than_64_assignments_and_fewer_agree(w4_bits):
+    """The groups are found two ways, one assignment a lane (12 tokens) or by a count (24)."""
+    w1, w2 = (v.to(DEV) for v in _half(32, 256, 128, BF, seed=43))
+    if w4_bits:
+        packs = dict(packed=w4.pack_w4_gate_up(*w4.quantize_w4(w1, 64)), packed_down=w4.pack_w4(*w4.quantize_w4(w2, 64)))
+        w1 = w2 = None
+    else:
+        packs = {}
+    x = torch.randn(24, 256, generator=torch.Generator().manual_seed(44)).to(BF).to(DEV)
+    ids, weights = (v.to(DEV) for v in _routing(24, 4, 32, seed=45))
+    want = torch.cat([moe.fused_moe(x[i:i + 12], ids[i:i + 12], weights[i:i + 12], w1, w2, **packs) for i in (0, 12)])
+    got = moe.fused_moe(x, ids, weights, w1, w2, **packs)
+    # the order of a token's choices may differ with the groups': fp32 sums of 4 terms, then one rounding
+    assert float((got.float() - want.float()).abs().max()) <= 2 * half_ulp(BF) * float(want.float().abs().max())
+
+
+def test_two_threads_on_one_stream():
+    """A call is two launches: each host thread has a workspace of its own."""
+    import threading
+    w1, w2 = (v.to(DEV) for v in _half(16, 512, 256, BF, seed=61))
+    ids, weights = (v.to(DEV) for v in _routing(8, 4, 16, seed=62))
+    xs = [torch.randn(8, 512, generator=torch.Generator().manual_seed(63 + i)).to(BF).to(DEV) for i in range(2)]
+    want = [moe.fused_moe(x, ids, weights, w1, w2) for x in xs]
+    got = [[], []]
+    threads = [threading.Thread(target=lambda i=i: got[i].extend(moe.fused_moe(xs[i], ids, weights, w1, w2) for _ in range(50)))
+               for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(len(g) == 50 and all(torch.equal(o, want[i]) for o in g) for i, g in enumerate(got))
+
+
+def test_captured_before_any_eager_call_on_its_stream():
+    w1, w2 = (v.to(DEV) for v in _half(8, 256, 128, BF, seed=64))
+    q = dict(packed=w4.pack_w4_gate_up(*w4.quantize_w4(w1, 32)), packed_down=w4.pack_w4(*w4.quantize_w4(w2, 64)))
+    ids, weights = (v.to(DEV) for v in _routing(5, 3, 8, seed=65))
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(66)).to(BF).to(DEV)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        half = moe.fused_moe(x, ids, weights, w1, w2)
+        four = moe.fused_moe(x, ids, weights, None, None, **q)
+    for i in range(3):
+        x.copy_(x + 0.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(half, moe.fused_moe(x, ids, weights, w1, w2))
+        assert torch.equal(four, moe.fused_moe(x, ids, weights, None, None, **q))
+
+
 def test_two_streams():
     """Calls on two streams at once have workspaces of their own."""
     w1, w2 = (v.to(DEV) for v in _half(16, 1024, 256, BF, seed=19))
