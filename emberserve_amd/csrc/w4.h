@@ -14,7 +14,8 @@
 // with sum x over the group from one more MFMA against ones, shared by all rows of the wave. The
 // terms are at most 31 / 8 times the size of the products they stand for, so the subtraction costs
 // 2 bits of fp32's 24; the scale is applied to the fp32 difference, once per group. No product is
-// rounded to 16 bits. An infinite x gives NaN (inf - inf) where the formula's sum would be infinite.
+// rounded to 16 bits. An infinite x, or one so large that a
+// group's sum of 31 x overflows fp32 (bf16, 2^116 and more), gives NaN (inf - inf) or an infinity.
 //
 // Packed layout: per expert, slabs of 16 rows (gate_up: gate slab 0, up slab 0, gate slab 1, ...). A slab
 // is nb = ceil(K / 128) blocks of 1 KiB of codes, then the scales of all blocks, rounded up to 128 bytes:

@@ -339,7 +339,7 @@ int w4_call(const void* x, int64_t xs, const void* packed, int64_t group, int dt
             int64_t rows, int gate_up, const void* bias, void* out, int64_t os, void* stream) {
   if (tokens == 0 && sizes_ok(rows, k, group)) return EMBER_OK;
   if (x == nullptr || packed == nullptr || out == nullptr || tokens < 0 || tokens > (int64_t(1) << 21) ||
-      !sizes_ok(rows, k, group) || xs > (int64_t(1) << 24) || (dtype != EMBER_F16 && dtype != EMBER_BF16) || os < 0 || xs < 0)
+      !sizes_ok(rows, k, group) || xs > (int64_t(1) << 23) || (dtype != EMBER_F16 && dtype != EMBER_BF16) || os < 0 || xs < 0)
     return EMBER_EINVAL;
   if (!aligned16(x) || !aligned16(packed) || xs % 8 != 0) return EMBER_EALIGN;
   W4Args a{x, xs, static_cast<const uint8_t*>(packed), bias, out, os, static_cast<int>(tokens), static_cast<int>(k),
@@ -347,7 +347,16 @@ int w4_call(const void* x, int64_t xs, const void* packed, int64_t group, int dt
            static_cast<int>(cdiv(k, kW4Block)), 0, 1, gate_up, 0};
   const int gpb = w4_gpb(group);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == EMBER_F16 ? w4_run<_Float16>(a, gpb, s) : w4_run<__bf16>(a, gpb, s);
+  // A launch has at most 2^31 threads: a wave for each slab and 16 tokens, where there are so many.
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 25) / (a.slabs + kXcds)) * 16;
+  for (int64_t done = 0; done < tokens; done += most) {
+    a.x = static_cast<const uint16_t*>(x) + done * xs;
+    a.out = static_cast<uint16_t*>(out) + done * os;
+    a.T = static_cast<int>(std::min(most, tokens - done));
+    const int st = dtype == EMBER_F16 ? w4_run<_Float16>(a, gpb, s) : w4_run<__bf16>(a, gpb, s);
+    if (st != EMBER_OK) return st;
+  }
+  return EMBER_OK;
 }
 
 // ---- packing ----------------------------------------------------------------------------

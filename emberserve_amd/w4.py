@@ -14,7 +14,8 @@ weights of `moe.fused_moe`. x is fp16 or bf16, whatever the scales' dtype.
 
 Numerics: the codes enter MFMA as exact fp16/bf16 integers, the products are summed in fp32, a group's
 sum is scaled in fp32, and the result is rounded once; gate_up_silu_w4 does not round between the
-projection and the activation, as the 16-bit pair does. A row of x with an infinity gives NaN.
+projection and the activation, as the 16-bit pair does. A row of x with an infinity gives NaN, and so may
+one whose 31-fold sum over a group overflows fp32 (bf16 values of 2^116 and more).
 
 A pass over the weight serves 64 tokens; more tokens take more passes, so at prefill sizes
 `PackedW4.dequantize` and a library GEMM are the faster way. CPU tensors, or `EMBERSERVE_FUSED_OPS=0`, take
@@ -31,7 +32,7 @@ from . import _lib
 from .ops import _launch, fused_enabled
 
 SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
-MAX_ROW_STRIDE = 1 << 24  # elements: a tile of tokens is addressed with 32-bit offsets
+MAX_ROW_STRIDE = 1 << 23  # elements: 64 tokens are addressed with 32-bit offsets; rows farther apart are copied
 
 
 def quantize_w4(weight: Tensor, group_size: int = 128, *, symmetric: bool = True) -> tuple[Tensor, Tensor, Tensor | None]:
@@ -44,7 +45,9 @@ def quantize_w4(weight: Tensor, group_size: int = 128, *, symmetric: bool = True
     k = weight.shape[-1]
     _check_group(k, group_size)
     w = weight.float().reshape(*weight.shape[:-1], k // group_size, group_size)
-    tiny = torch.finfo(weight.dtype).tiny  # a group of zeros: any scale, codes at the zero point
+    # a group of zeros: any scale, codes at the zero point. fp16 weights under 2^-11 have scales below
+    # its normal range, whose smallest step is 2^-24
+    tiny = 2.0 ** -24 if weight.dtype == torch.float16 else torch.finfo(weight.dtype).tiny
     if symmetric:
         scales = (w.abs().amax(-1) / 7.0).clamp_min(tiny).to(weight.dtype)
         zero = torch.full_like(scales, 8.0, dtype=torch.float32)

@@ -641,8 +641,9 @@ int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t 
 
 /* out[t, n] = round(x[t] . w[n] + bias[n]) over a packed 4-bit weight, x [tokens, k] and out
  * [tokens, rows] fp16 or bf16 (dtype), bias [rows] of that dtype or NULL. Unit inner strides; x 16-byte
- * aligned with a row stride that is a multiple of 8 (EMBER_EALIGN otherwise). Sums are fp32, rounded
- * once. Any number of tokens up to 2^21; 64 of them share a pass over the weight. */
+ * aligned with a row stride that is a multiple of 8 (EMBER_EALIGN otherwise) and at most 2^23. Sums are
+ * fp32, rounded once. Any number of tokens up to 2^21; up to 64 of them share a pass over the weight, and more
+ * than 2^33 outputs take several launches. */
 int ember_w4_linear(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype, int64_t tokens,
                     int64_t k, int64_t rows, const void* bias, void* out, int64_t out_row_stride, void* stream);
 
@@ -663,7 +664,8 @@ int ember_w4_gate_up_silu(const void* x, int64_t x_row_stride, const void* packe
  * experts gets zeros. w_gate_up [num_experts, 2 inter, hidden] (gate rows, then up rows) and w_down
  * [num_experts, hidden, inter], of dtype, by strides; a row stride of 0 marks the packed forms of
  * ember_moe_gate_up_silu_pack_weight and ember_moe_down_pack_weight. hidden and inter multiples of
- * 64, num_experts <= 1024; x and weights 16-byte aligned, strides multiples of 8 (EMBER_EALIGN).
+ * 64 up to 2^18, num_experts <= 1024; x and weights 16-byte aligned, strides multiples of 8
+ * (EMBER_EALIGN), x's at most 2^23.
  * The workspace (ember_moe_layer_workspace_bytes; more is fine, the size a multiple of 16) holds
  * counters at its end, *counter_bytes of them, which must be zero before its first use and are left
  * zero; calls of different shapes may take turns on one workspace as long as no call's other part

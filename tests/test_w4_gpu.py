@@ -142,6 +142,97 @@ def test_extreme_scales_and_values():
     assert bool(got.cpu()[over].isinf().all())
 
 
+def test_tiny_and_large_values():
+    """Subnormal x beside ordinary ones (each token its own size), and bf16 x as large as the sums hold."""
+    for dtype, sizes in ((HF, (2.0 ** -24, 2.0 ** -20, 2.0 ** -14, 1.0)), (BF, (2.0 ** -130, 2.0 ** -100, 1.0, 2.0 ** 110))):
+        parts = _weight(64, 256, 64, True, HF, seed=24)  # fp16 scales under either type of x
+        x = torch.stack([_x(1, 256, torch.float32, seed=30 + i)[0] * v for i, v in enumerate(sizes)]).to(dtype)
+        w, s = codes64(*parts)
+        want, bound = dot_bound(x, w, s, 64)
+        got = w4.linear_w4(x.to(DEV), w4.pack_w4(*_dev(parts)))
+        # fp32 sums of such products may themselves be subnormal: 2^-149 a rounding
+        check(got, want, bound + 400 * 2.0 ** -149, f"{dtype}")
+
+
+def test_overlapping_rows():
+    """One token for all rows, by a row stride of zero, and rows that overlap."""
+    packed = w4.pack_w4(*_dev(_weight(48, 256, 64, False, BF, seed=25)))
+    flat = _x(1, 512, BF, seed=26).to(DEV)[0]
+    one = flat[:256].expand(9, 256)
+    assert torch.equal(w4.linear_w4(one, packed), w4.linear_w4(one.contiguous(), packed))
+    slide = flat.as_strided((20, 256), (8, 1))
+    assert torch.equal(w4.linear_w4(slide, packed), w4.linear_w4(slide.contiguous(), packed))
+
+
+@pytest.mark.parametrize("t,n,k", [(2000, 160, 256), (777, 40, 1056), (300, 24576, 128)])
+def test_many_tokens(t, n, k):
+    """Prefill-sized batches: many tiles of tokens, the last one ragged."""
+    parts = _weight(n, k, 32, True, BF, seed=50)
+    x = _x(t, k, BF, seed=51)
+    w, s = codes64(*parts)
+    rows = torch.cat((torch.arange(0, t, 37), torch.arange(t - 40, t)))
+    want, bound = dot_bound(x[rows], w, s, 32)
+    got = w4.linear_w4(x.to(DEV), w4.pack_w4(*_dev(parts)))
+    check(got[rows.to(DEV)], want, bound)
+
+
+def test_rows_far_apart_are_copied():
+    """Row strides past what 32-bit offsets reach over 64 rows."""
+    parts = _weight(48, 128, 64, False, BF, seed=52)
+    packed = w4.pack_w4(*_dev(parts))
+    stride = w4.MAX_ROW_STRIDE + 8
+    big = torch.zeros(2 * stride + 128, dtype=BF, device=DEV)
+    x = big.as_strided((3, 128), (stride, 1))
+    x.copy_(_x(3, 128, BF, seed=53))
+    assert torch.equal(w4.linear_w4(x, packed), w4.linear_w4(x.contiguous(), packed))
+
+
+def test_rows_at_the_largest_stride():
+    """64 rows at the largest stride that is read in place: offsets up to 2^30."""
+    parts = _weight(32768, 128, 64, False, BF, seed=54)
+    stride = w4.MAX_ROW_STRIDE
+    big = torch.zeros(63 * stride + 128, dtype=BF, device=DEV)
+    x = big.as_strided((64, 128), (stride, 1))
+    x.copy_(_x(64, 128, BF, seed=55))
+    for sub in (parts, tuple(None if p is None else p[:48] for p in parts)):
+        packed = w4.pack_w4(*_dev(sub))
+        assert torch.equal(w4.linear_w4(x, packed), w4.linear_w4(x.contiguous(), packed))
+
+
+def test_more_threads_than_one_launch_takes():
+    """2^23 slabs of 16 rows: 64 tokens a launch, the 66 take two."""
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GiB of device memory")
+    slabs = (1 << 23) - 8
+    q = torch.randint(0, 256, (slabs * 16, 16), dtype=torch.uint8, device=DEV)
+    s = torch.ones(slabs * 16, 1, dtype=BF, device=DEV)
+    packed = w4.pack_w4(q, s)
+    g = torch.Generator().manual_seed(60)
+    x = torch.randint(-4, 5, (66, 32), generator=g).to(BF).to(DEV)  # sums of whole numbers, exact in fp32
+    got = w4.linear_w4(x, packed)
+    n = slabs * 16
+    some = torch.cat((torch.arange(64), torch.randint(0, n, (256,), generator=g), torch.arange(n - 64, n))).to(DEV)
+    codes = torch.stack((q[some] & 15, q[some] >> 4), -1).reshape(-1, 32).float() - 8
+    assert torch.equal(got[:, some], (x.float() @ codes.T).to(BF))
+
+
+def test_two_threads_on_one_stream():
+    """Calls of two host threads, each into its own output."""
+    import threading
+    parts = _weight(256, 1024, 128, False, BF, seed=56)
+    packed = w4.pack_w4(*_dev(parts))
+    xs = [_x(5 + 8 * i, 1024, BF, seed=57 + i).to(DEV) for i in range(2)]
+    want = [w4.linear_w4(x, packed) for x in xs]
+    got = [[], []]
+    threads = [threading.Thread(target=lambda i=i: got[i].extend(w4.linear_w4(xs[i], packed) for _ in range(50)))
+               for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(len(g) == 50 and all(torch.equal(o, want[i]) for o in g) for i, g in enumerate(got))
+
+
 def test_graph_replays_match_eager():
     parts, gu = _weight(1152, 896, 128, False, BF, seed=10), _weight(2 * 304, 896, 128, False, BF, seed=11)
     packed, packed_gu = w4.pack_w4(*_dev(parts)), w4.pack_w4_gate_up(*_dev(gu))

@@ -38,6 +38,19 @@ def test_quantize_rounds_to_nearest(dtype, symmetric, group):
     assert bool((d[3, :group] == 0).all())
 
 
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantize_small_fp16_weights(symmetric):
+    """Scales below fp16's normal range are multiples of 2^-24: half of one more a code for the scale's
+    rounding, which may also put the ends of the range out of the codes' reach, by as much."""
+    w = (_w(16, 256, torch.float32, seed=70) * 2.0 ** -10).to(HF)
+    q, s, z = w4.quantize_w4(w, 64, symmetric=symmetric)
+    assert float(s.max()) < torch.finfo(HF).tiny
+    d = w4.dequantize_w4(q, s, z, dtype=torch.float32)
+    step = s.double().repeat_interleave(64, -1)
+    slack = (7 if symmetric else 15) * 2.0 ** -25 + (0 if symmetric else 0.5) * step
+    assert bool(((d.double() - w.double()).abs() <= 0.5 * step * (1 + 1e-6) + slack).all())
+
+
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
 def test_eager_forms_match_64_bits(group, zeros):
     parts = w4.quantize_w4(_w(60, 384, BF), group, symmetric=not zeros)
