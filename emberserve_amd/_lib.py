@@ -113,6 +113,8 @@ SIGNATURES: dict[str, list] = {
     "ember_w4_pack_weight": [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p,
                              _p],
     "ember_w4_linear": [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _i64, _p],
+    "ember_w4_linear_workspace_bytes": [_i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "ember_w4_linear_split": [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p],
     "ember_w4_gate_up_silu": [_p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _p, _i64, _p],
     "ember_moe_layer_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "ember_moe_layer": [_p, _i64, _p, _i32, _p, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64,
@@ -131,6 +133,7 @@ _RESTYPE = {"ember_status_string": ctypes.c_char_p, "ember_paged_decode_workspac
             "ember_gate_up_silu_workspace_bytes": ctypes.c_int64,
             "ember_moe_gate_up_silu_workspace_bytes": ctypes.c_int64,
             "ember_w4_packed_bytes": ctypes.c_int64,
+            "ember_w4_linear_workspace_bytes": ctypes.c_int64,
             "ember_moe_layer_workspace_bytes": ctypes.c_int64,
             "ember_moe_align_padded_size": ctypes.c_int64,
             "ember_moe_align_workspace_bytes": ctypes.c_int64,

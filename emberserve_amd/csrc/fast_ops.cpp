@@ -45,14 +45,14 @@ struct Entry {
 };
 enum {
   kRmsnorm, kAddRmsnorm, kRope, kSilu, kEmbedding, kQkNormRope, kMlaLatentRope, kRopeKvCache, kMlaLatentRopeCache,
-  kPagedDecode, kMlaDecode, kW4Linear, kW4GateUp, kMoeLayer, kMoeLayerW4, kStatusString, kEntries
+  kPagedDecode, kMlaDecode, kW4Space, kW4Linear, kW4GateUp, kMoeLayer, kMoeLayerW4, kStatusString, kEntries
 };
 Entry g_entry[kEntries] = {
     {"ember_rmsnorm", nullptr}, {"ember_fused_add_rmsnorm", nullptr}, {"ember_rope", nullptr},
     {"ember_silu_and_mul", nullptr}, {"ember_embedding", nullptr}, {"ember_qk_norm_rope", nullptr},
     {"ember_mla_latent_rope", nullptr}, {"ember_rope_kv_cache", nullptr}, {"ember_mla_latent_rope_cache", nullptr},
     {"ember_paged_decode_shared", nullptr}, {"ember_mla_decode", nullptr},
-    {"ember_w4_linear", nullptr}, {"ember_w4_gate_up_silu", nullptr}, {"ember_moe_layer", nullptr},
+    {"ember_w4_linear_workspace_bytes", nullptr}, {"ember_w4_linear_split", nullptr}, {"ember_w4_gate_up_silu", nullptr}, {"ember_moe_layer", nullptr},
     {"ember_moe_layer_w4", nullptr}, {"ember_status_string", nullptr}};
 bool g_bound = false;
 
@@ -593,10 +593,11 @@ bool as_ints(PyObject* o, int64_t (&v)[N]) {
   return true;
 }
 
-// (x, packed, bias or None, (rows, k, group, gate_up)) -> out. The tuple is the packed weight's own.
+// (x, packed, bias or None, (rows, k, group, gate_up), plan) -> out. The tuple is the packed weight's own; the
+// plan is called for a workspace only where the call needs one.
 PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 4) Py_RETURN_NONE;
+  if (n != 5) Py_RETURN_NONE;
   Call c;
   const at::Tensor* x = c.tensor(a[0]);
   const at::Tensor* w = c.tensor(a[1]);
@@ -612,6 +613,12 @@ PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
   sizes.back() = rows;
+  Plan p;
+  if (shape[3] == 0) {
+    int64_t counters = 0;
+    const int64_t need = ENTRY(kW4Space, ember_w4_linear_workspace_bytes)(r.rows, k, rows, group, &counters);
+    if (need > 0 && !p.resolve(a[4], {need, counters}, a[0])) return nullptr;
+  }
   at::Tensor out = at::empty(sizes, x->options());
   void* s = c.stream();
   const int entry = shape[3] != 0 ? kW4GateUp : kW4Linear;
@@ -619,9 +626,9 @@ PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return entry == kW4GateUp
                ? ENTRY(kW4GateUp, ember_w4_gate_up_silu)(x->data_ptr(), r.stride, w->data_ptr(), group, tag, r.rows, k,
                                                          rows, out.data_ptr(), rows, s)
-               : ENTRY(kW4Linear, ember_w4_linear)(x->data_ptr(), r.stride, w->data_ptr(), group, tag, r.rows, k, rows,
-                                                   bias != nullptr ? bias->data_ptr() : nullptr, out.data_ptr(), rows,
-                                                   s);
+               : ENTRY(kW4Linear, ember_w4_linear_split)(x->data_ptr(), r.stride, w->data_ptr(), group, tag, r.rows, k,
+                                                         rows, bias != nullptr ? bias->data_ptr() : nullptr, p.ws,
+                                                         p.ws_bytes, out.data_ptr(), rows, s);
   });
   if (!answered(st, entry)) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

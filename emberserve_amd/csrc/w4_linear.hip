@@ -26,24 +26,32 @@ struct W4Args {
   int tiles;     // sets of 16 NT tokens
   int gate_up;
   int side;      // k_w4_wide: waves side by side
+  int splits;    // k_w4_linear: workgroups that share a set's k, ...
+  float* part;   // ... their sums [group][tile][split][nt R + r][lane][4] (null: no splits)
+  uint32_t* counters;  // and arrivals [group][tile]
 };
 
 constexpr int kXcds = 8;
+constexpr int kW4MaxSplits = 8;
+constexpr int kSplitTokens = 64;  // most tokens whose k is split: more fill the chip
 
-// A workgroup holds R slabs against NT tiles of 16 tokens (XI < 4: of 4 XI); its waves share k, block by
-// block. D blocks in flight a wave.
+// A workgroup holds R slabs against NT tiles of 16 tokens (XI < 4: of 4 XI); its waves, and those of the
+// other splits, share k, block by block. D blocks in flight a wave.
 template <typename T, int R, int GPB, int NT, int XI, int D, int MAXW>
 __global__ void __launch_bounds__(MAXW * kWave)
 k_w4_linear(W4Args a) {
   using X = XBlock<NT, XI>;
   constexpr int P = X::kPieces > 64 * R * NT ? X::kPieces : 64 * R * NT;
   extern __shared__ __attribute__((aligned(16))) u32x4 lds[];  // [wave][P]: a block's tokens, then the sums
+  __shared__ int last;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = blockDim.x >> 6;
   // the tiles of a slab group on one XCD, next to each other: its L2 holds the weights for them
-  const int per = kXcds * a.tiles;
-  const int tile = blockIdx.x % per / kXcds;
+  const int per = kXcds * a.tiles * a.splits;
+  const int sub = blockIdx.x % per / kXcds;
+  const int split = a.splits > 1 ? sub / a.tiles : 0, tile = sub - split * a.tiles;
+  const int first = split * wk + wave, stride = a.splits * wk;
   const int group = blockIdx.x / per * kXcds + blockIdx.x % kXcds;
   if (group >= a.groups) return;
   const int slab0 = group * R, tok0 = 16 * NT * tile;
@@ -71,9 +79,9 @@ k_w4_linear(W4Args a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[nt][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   stream<Stage, D>(
-      0, wave < a.nb ? (a.nb - wave + wk - 1) / wk : 0,
+      0, first < a.nb ? (a.nb - first + stride - 1) / stride : 0,
       [&](Stage& g, int j) {
-        const int b = min(wave + j * wk, a.nb - 1);
+        const int b = min(first + j * stride, a.nb - 1);
 #pragma unroll
         for (int r = 0; r < R; ++r) g.w.load(r, base[r], b, a.nb, lane);
         g.x.load(xr, off, b, a.K, lane);
@@ -96,12 +104,12 @@ k_w4_linear(W4Args a) {
       static_cast<T*>(a.out)[static_cast<int64_t>(tok0 + tok) * a.os + col] = from_f32<T>(y);
     }
   };
-  if (wk == 1) {
+  if (wk == 1 && a.splits == 1) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (r % 2 == 0 || !a.gate_up) emit(nt, slab0 + r, acc[nt][r], acc[nt][R > 1 ? r | 1 : r]);
+        if (r % 2 == 0 || !a.gate_up) emit(nt, slab0 + r, acc[nt][r], acc[nt][(r | 1) < R ? r | 1 : r]);
     return;
   }
   // the waves take the tiles (gate and up together) in turn, summing the waves' shares of k in order
@@ -117,6 +125,33 @@ k_w4_linear(W4Args a) {
     for (int q = 1; q < wk; ++q) v += red[q * P + t * kWave + lane];
     return v;
   };
+  if (a.splits > 1) {  // not gate_up
+    const int set = group * a.tiles + tile;
+    constexpr int kSums = NT * R * kWave;
+    const CoherentRsrc rs =
+        coherent_rsrc(a.part + static_cast<int64_t>(set) * a.splits * kSums * 4, a.splits * kSums * 4);
+    for (int t = wave; t < NT * R; t += wk) store_coherent<4>(rs, (split * kSums + t * kWave + lane) * 16, total(t));
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const uint32_t prev = __hip_atomic_fetch_add(a.counters + set, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = prev == static_cast<uint32_t>(a.splits) - 1;
+      if (last) __hip_atomic_store(a.counters + set, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int t = wave; t < NT * R; t += wk) {  // in the splits' order, whoever is last
+      f32x4 v[kW4MaxSplits];
+#pragma unroll
+      for (int s = 0; s < kW4MaxSplits; ++s)
+        v[s] = load_coherent<4>(rs, (min(s, a.splits - 1) * kSums + t * kWave + lane) * 16);
+      f32x4 y = v[0];
+#pragma unroll
+      for (int s = 1; s < kW4MaxSplits; ++s) y += s < a.splits ? v[s] : f32x4{0.f, 0.f, 0.f, 0.f};
+      emit(t / R, slab0 + t % R, y, y);
+    }
+    return;
+  }
   const int step = a.gate_up ? 2 : 1;
   for (int t = wave * step; t < NT * R; t += wk * step) {
     const f32x4 v = total(t);
@@ -258,33 +293,48 @@ int w4_launch(W4Args a, hipStream_t stream) {
   const int64_t cus = std::max(1, device_cu_count());
   a.groups = static_cast<int>(cdiv(a.slabs, R));
   a.tiles = static_cast<int>(cdiv(a.T, 16 * NT));
-  const int64_t grid = cdiv(a.groups, kXcds) * kXcds * a.tiles;
+  const int64_t grid = cdiv(a.groups, kXcds) * kXcds * a.tiles * a.splits;
   // Waves along k: 7 or more a CU, each with at least a block or two. Measured (us): Qwen2.5-7B down, 2
   // tokens (224 slabs, 148 blocks) 12.6 with 4, 11.8 with 8, 13.6 with 16; Qwen3-8B head, 16 tokens (2374
   // sets of slabs) 70.4 with 1, 75.6 with 2.
   int wk = 1;
-  while (wk < MAXW && grid * wk < 7 * cus && 2 * wk < a.nb) wk *= 2;
+  while (wk < MAXW && grid * wk < 7 * cus && 2 * wk * a.splits < a.nb) wk *= 2;
   const size_t lds = size_t(wk) * 16 * std::max(XBlock<NT, XI>::kPieces, 64 * R * NT);
   k_w4_linear<T, R, GPB, NT, XI, D, MAXW><<<dim3(static_cast<unsigned>(grid)), wk * kWave, lds, stream>>>(a);
   return launch_status();
 }
 
-// Slabs a workgroup: more of them share a block's tokens, whose loads take about as long as one slab's, but
-// fewer workgroups fill the chip. The number with the shortest rounds. Measured (us at 1 | 2 | 4 slabs):
-// 256 slabs x 4096, 16 tokens 6.8 | 7.8 | 11.1; 384 x 4096, 16 tokens 9.2 | 8.0 | 11.3, 64 tokens 18.2 | 16.7
-// | 12.5; gate_up 1536 x 4096, 16 tokens 2 | 4: 18.3 | 21.9, 64 tokens 35.1 | 31.6.
-int w4_slabs(const W4Args& a, int tokens) {
-  const int64_t cus = std::max(1, device_cu_count()), tiles = cdiv(a.T, tokens);
-  int best = 0;
+// Slabs a workgroup and splits of k. More slabs share a block's tokens, but fewer workgroups fill the chip,
+// unless several split the slabs' k and join their sums. The choice with the shortest rounds: a block is 1 KiB
+// a slab at the 24 GB/s that a CU takes in from memory, and XI NT KiB of tokens at three times that from L2;
+// a join costs 3 us, what 80 KiB from memory do. Splits that only even out the last round lose: the head's 9496
+// slabs x 4096, 16 tokens 4/1 64.5, 4/2 82.6. Measured (us at slabs/splits): 256 slabs x 4096, 16 tokens
+// 1/1 7.5, 2/1 8.6, 4/4 9.7; 384 x 4096, 16 tokens 2/1 8.0, 1/1 10.3, 61 tokens 3/1 12.3, 4/1 13.1, 2/2 15.1;
+// 224 x 18944, 6 tokens 1/1 13.1, 4/4 13.4, 16 tokens 4/4 14.9, 1/1 16.9, 24 tokens 4/4 17.1, 2/2 18.9, 1/1 23.7,
+// 61 tokens 4/2 25.3, 2/1 29.0; gate_up 1536 x 4096, 16 tokens 2/1 18.3, 4/1 21.9, 64 tokens 4/1 31.6, 2/1 35.1.
+struct W4Shape {
+  int r, splits;
+};
+W4Shape w4_shape(const W4Args& a, int nt, int xi, bool split) {
+  const int64_t cus = std::max(1, device_cu_count()), tiles = cdiv(a.T, 16 * nt);
+  W4Shape best{0, 1};
   int64_t least = 0;
-  for (int r = a.gate_up ? 2 : 1; r <= 4; r *= 2) {
-    const int64_t cost = cdiv(cdiv(a.slabs, r) * tiles, cus) * (r + 1);
-    if (best == 0 || cost < least) {
-      best = r;
-      least = cost;
+  for (int s = 1; s == 1 || (split && s <= kW4MaxSplits && 8 * s <= a.nb); ++s)
+    for (int r = a.gate_up ? 2 : 1; r <= 4; r += a.gate_up ? 2 : 1) {
+      const int64_t wgs = cdiv(a.slabs, r) * tiles * s;
+      if (s > 1 && wgs > 2 * cus) continue;  // the chip is full without
+      const int64_t cost =
+          cdiv(wgs, cus) * cdiv(a.nb, s) * (3 * r + xi * nt) + (s > 1 ? 3 * 80 : 0);
+      if (best.r == 0 || cost < least) {
+        best = {r, s};
+        least = cost;
+      }
     }
-  }
   return best;
+}
+// The same of a call, for w4_pick and for the size of its workspace.
+W4Shape w4_shape(const W4Args& a, bool split) {
+  return w4_shape(a, a.T <= 16 ? 1 : 2, a.T <= 8 ? 2 : 4, split && !a.gate_up && a.T <= kSplitTokens);
 }
 
 // Token tiles, slabs and depth by size. Two tiles a wave from 17 tokens: the codes are turned into operands
@@ -301,19 +351,24 @@ int w4_pick(W4Args a, hipStream_t stream) {
     a.side = side;
     return wide_pick<T, GPB>(a, stream);
   }
-  const int r = w4_slabs(a, a.T <= 16 ? 16 : 32);
+  const W4Shape shape = w4_shape(a, a.part != nullptr);
+  const int r = shape.r;
+  a.splits = shape.splits;
   if (a.T <= 8) {
     if (r == 1) return w4_launch<T, 1, GPB, 1, 2, 4, 16>(a, stream);
     if (r == 2) return w4_launch<T, 2, GPB, 1, 2, 4, 8>(a, stream);
+    if (r == 3) return w4_launch<T, 3, GPB, 1, 2, 3, 8>(a, stream);
     return w4_launch<T, 4, GPB, 1, 2, 3, 8>(a, stream);
   }
   if (a.T <= 16) {
     if (r == 1) return w4_launch<T, 1, GPB, 1, 4, GPB == 1 ? 4 : 3, 16>(a, stream);
     if (r == 2) return w4_launch<T, 2, GPB, 1, 4, 4, 8>(a, stream);
+    if (r == 3) return w4_launch<T, 3, GPB, 1, 4, 3, 8>(a, stream);
     return w4_launch<T, 4, GPB, 1, 4, 3, 8>(a, stream);
   }
   if (r == 1) return w4_launch<T, 1, GPB, 2, 4, 3, 8>(a, stream);
   if (r == 2) return w4_launch<T, 2, GPB, 2, 4, 2, 8>(a, stream);
+  if (r == 3) return w4_launch<T, 3, GPB, 2, 4, 2, 8>(a, stream);
   return w4_launch<T, 4, GPB, 2, 4, 2, 8>(a, stream);
 }
 
@@ -335,16 +390,53 @@ bool sizes_ok(int64_t rows, int64_t k, int64_t group) {
   return rows >= 1 && rows <= (int64_t(1) << 27) && k >= 32 && k <= (int64_t(1) << 24) && group_ok(k, group);
 }
 
+struct W4Space {
+  int64_t part, counters;  // bytes
+};
+// What a call's splits need: nothing for most.
+W4Space w4_space(const W4Args& a) {
+  if (a.T <= 4 || a.T > kSplitTokens || a.gate_up || wide_side(a) != 0) return {0, 0};
+  const W4Shape s = w4_shape(a, true);
+  if (s.splits == 1) return {0, 0};
+  const int nt = a.T <= 16 ? 1 : 2;
+  const int64_t sets = cdiv(a.slabs, s.r) * cdiv(a.T, 16 * nt);
+  return {sets * s.splits * nt * s.r * kWave * 16, cdiv(sets * 4, 256) * 256};
+}
+
+W4Args w4_args(int64_t tokens, int64_t k, int64_t rows, int gate_up) {
+  W4Args a{};
+  a.T = static_cast<int>(tokens);
+  a.K = static_cast<int>(k);
+  a.N = static_cast<int>(rows);
+  a.slabs = static_cast<int>(cdiv(rows, 16)) * (gate_up ? 2 : 1);
+  a.nb = static_cast<int>(cdiv(k, kW4Block));
+  a.tiles = a.splits = 1;
+  a.gate_up = gate_up;
+  return a;
+}
+
 int w4_call(const void* x, int64_t xs, const void* packed, int64_t group, int dtype, int64_t tokens, int64_t k,
-            int64_t rows, int gate_up, const void* bias, void* out, int64_t os, void* stream) {
+            int64_t rows, int gate_up, const void* bias, void* workspace, int64_t workspace_bytes, void* out,
+            int64_t os, void* stream) {
   if (tokens == 0 && sizes_ok(rows, k, group)) return EMBER_OK;
   if (x == nullptr || packed == nullptr || out == nullptr || tokens < 0 || tokens > (int64_t(1) << 21) ||
       !sizes_ok(rows, k, group) || xs > (int64_t(1) << 23) || (dtype != EMBER_F16 && dtype != EMBER_BF16) || os < 0 || xs < 0)
     return EMBER_EINVAL;
   if (!aligned16(x) || !aligned16(packed) || xs % 8 != 0) return EMBER_EALIGN;
-  W4Args a{x, xs, static_cast<const uint8_t*>(packed), bias, out, os, static_cast<int>(tokens), static_cast<int>(k),
-           static_cast<int>(rows), static_cast<int>(cdiv(rows, 16)) * (gate_up ? 2 : 1),
-           static_cast<int>(cdiv(k, kW4Block)), 0, 1, gate_up, 0};
+  W4Args a = w4_args(tokens, k, rows, gate_up);
+  a.xs = xs;
+  a.w = static_cast<const uint8_t*>(packed);
+  a.bias = bias;
+  a.os = os;
+  if (workspace != nullptr) {
+    if (!aligned16(workspace) || workspace_bytes % 16 != 0) return EMBER_EALIGN;
+    const W4Space need = w4_space(a);
+    if (workspace_bytes < need.part + need.counters) return EMBER_EINVAL;
+    if (need.part > 0) {
+      a.part = static_cast<float*>(workspace);
+      a.counters = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + workspace_bytes - need.counters);
+    }
+  }
   const int gpb = w4_gpb(group);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // A launch has at most 2^31 threads: a wave for each slab and 16 tokens, where there are so many.
@@ -452,13 +544,28 @@ int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t 
 
 int ember_w4_linear(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype, int64_t tokens,
                     int64_t k, int64_t rows, const void* bias, void* out, int64_t out_row_stride, void* stream) {
-  return w4_call(x, x_row_stride, packed, group, dtype, tokens, k, rows, 0, bias, out, out_row_stride, stream);
+  return w4_call(x, x_row_stride, packed, group, dtype, tokens, k, rows, 0, bias, nullptr, 0, out, out_row_stride, stream);
+}
+
+int64_t ember_w4_linear_workspace_bytes(int64_t tokens, int64_t k, int64_t rows, int64_t group, int64_t* counter_bytes) {
+  if (tokens < 0 || tokens > (int64_t(1) << 21) || !sizes_ok(rows, k, group)) return -1;
+  const W4Space s = w4_space(w4_args(tokens, k, rows, 0));
+  if (counter_bytes != nullptr) *counter_bytes = s.counters;
+  return s.part + s.counters;
+}
+
+int ember_w4_linear_split(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype,
+                          int64_t tokens, int64_t k, int64_t rows, const void* bias, void* workspace,
+                          int64_t workspace_bytes, void* out, int64_t out_row_stride, void* stream) {
+  return w4_call(x, x_row_stride, packed, group, dtype, tokens, k, rows, 0, bias, workspace, workspace_bytes, out,
+                 out_row_stride, stream);
 }
 
 int ember_w4_gate_up_silu(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype,
                           int64_t tokens, int64_t hidden, int64_t inter, void* out, int64_t out_row_stride,
                           void* stream) {
-  return w4_call(x, x_row_stride, packed, group, dtype, tokens, hidden, inter, 1, nullptr, out, out_row_stride, stream);
+  return w4_call(x, x_row_stride, packed, group, dtype, tokens, hidden, inter, 1, nullptr, nullptr, 0, out, out_row_stride,
+                 stream);
 }
 
 }  // extern "C"

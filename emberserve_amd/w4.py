@@ -24,12 +24,15 @@ the eager forms.
 
 from __future__ import annotations
 
+from ctypes import byref, c_int64
+
 import torch
 import torch.nn.functional as F
 from torch import Tensor
 
 from . import _lib
-from .ops import _launch, fused_enabled
+from ._scratch import SharedScratch
+from .ops import _check_indices, _launch, fused_enabled
 
 SUPPORTED_DTYPES = (torch.float16, torch.bfloat16)
 MAX_ROW_STRIDE = 1 << 23  # elements: 64 tokens are addressed with 32-bit offsets; rows farther apart are copied
@@ -194,10 +197,20 @@ def _rows(x: Tensor) -> Tensor:
     return x2
 
 
+# Sums and arrival counters of calls whose k is split over workgroups: one buffer per (thread, device,
+# stream), and one per graph capture.
+_SCRATCH = SharedScratch("linear_w4", per_capture=True)
+
+
+def _workspace(need: int, counters: int, x: Tensor) -> tuple[int, Tensor]:
+    """(0, a workspace of `need` bytes, `counters` of them at its end)."""
+    return 0, _SCRATCH.get(need - counters, counters, x.device)
+
+
 def linear_w4(x: Tensor, weight: PackedW4, bias: Tensor | None = None) -> Tensor:
     """round(x @ w.T + bias) [..., N] over a weight from `pack_w4`; bias [N] of x's dtype or None."""
     if type(weight) is PackedW4 and weight.projection is not None and not weight.gate_up and not _lib.tracing():
-        got = _lib.fast.w4_linear(x, weight.packed, bias, weight.projection)
+        got = _lib.fast.w4_linear(x, weight.packed, bias, weight.projection, _workspace)
         if got is not None:  # an ordinary call, answered by the native host path
             return got
     _check("linear_w4", x, weight, False)
@@ -211,9 +224,18 @@ def linear_w4(x: Tensor, weight: PackedW4, bias: Tensor | None = None) -> Tensor
     if x2.shape[0]:
         if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
-        _launch("ember_w4_linear", _lib.load().ember_w4_linear, x.device, x2.data_ptr(), x2.stride(0),
+        lib, counters, ws = _lib.load(), c_int64(0), None
+        with torch.cuda.device(x.device):
+            need = lib.ember_w4_linear_workspace_bytes(x2.shape[0], weight.k, weight.rows, weight.group, byref(counters))
+        if need > 0:
+            ws = _workspace(need, counters.value, x)[1]
+        size = 0 if ws is None else ws.numel() * 4
+        _launch("ember_w4_linear_split", lib.ember_w4_linear_split, x.device, x2.data_ptr(), x2.stride(0),
                 weight.packed.data_ptr(), weight.group, _lib.dtype_tag(x.dtype), x2.shape[0], weight.k, weight.rows,
-                None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0))
+                None if bias is None else bias.data_ptr(), None if ws is None else ws.data_ptr(), size,
+                out.data_ptr(), out.stride(0))
+        if ws is not None and _check_indices():
+            _SCRATCH.verify_counters(ws, size - counters.value, size)
     return out.view(*x.shape[:-1], weight.rows)
 
 
@@ -221,7 +243,7 @@ def gate_up_silu_w4(x: Tensor, weight: PackedW4) -> Tensor:
     """round(silu(gate) * up) [..., I] over a weight from `pack_w4_gate_up`: `gate_up_silu` with 4-bit
     weights."""
     if type(weight) is PackedW4 and weight.projection is not None and weight.gate_up and not _lib.tracing():
-        got = _lib.fast.w4_linear(x, weight.packed, None, weight.projection)
+        got = _lib.fast.w4_linear(x, weight.packed, None, weight.projection, _workspace)
         if got is not None:
             return got
     _check("gate_up_silu_w4", x, weight, True)

@@ -647,6 +647,17 @@ int ember_w4_pack_weight(const void* codes, int64_t code_expert_stride, int64_t 
 int ember_w4_linear(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype, int64_t tokens,
                     int64_t k, int64_t rows, const void* bias, void* out, int64_t out_row_stride, void* stream);
 
+/* The same with a workspace, with which a few long rows' k is split over workgroups that join their sums
+ * (5 to 64 tokens). ember_w4_linear_workspace_bytes of the current device (0: no splits, and none is
+ * needed; more is fine, the size a multiple of 16): fp32 sums at its start and *counter_bytes of counters
+ * at its end, which must be zero before its first use and are left zero. Calls of different shapes may
+ * take turns on one workspace as long as no call's sums reach another's counters. NULL: as
+ * ember_w4_linear. */
+int64_t ember_w4_linear_workspace_bytes(int64_t tokens, int64_t k, int64_t rows, int64_t group, int64_t* counter_bytes);
+int ember_w4_linear_split(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype,
+                          int64_t tokens, int64_t k, int64_t rows, const void* bias, void* workspace,
+                          int64_t workspace_bytes, void* out, int64_t out_row_stride, void* stream);
+
 /* out[t, j] = round(silu(g) * u), g and u the fp32 products of x[t] with gate row j and up row j of a
  * weight packed with gate_up (rows = inter). Not rounded in between, unlike ember_gate_up_silu. */
 int ember_w4_gate_up_silu(const void* x, int64_t x_row_stride, const void* packed, int64_t group, int dtype,

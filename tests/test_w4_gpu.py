@@ -3,6 +3,9 @@ bounds of tests.w4_bounds."""
 
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import pytest
 import torch
 
@@ -176,6 +179,92 @@ def test_many_tokens(t, n, k):
     check(got[rows.to(DEV)], want, bound)
 
 
+def _need(t, k, n, group):
+    counters = ctypes.c_int64(0)
+    return _lib.load().ember_w4_linear_workspace_bytes(t, k, n, group, ctypes.byref(counters)), counters.value
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,n,k,group", [(24, 3584, 18944, 128), (61, 2056, 12288, 64), (17, 900, 4864, 32),
+                                         (33, 40, 8224, 32), (64, 16, 16384, 256), (16, 200, 20480, 128)])
+def test_long_rows_are_split(dtype, t, n, k, group):
+    """A few long rows: the workgroups that share k join their sums, the same bits each time."""
+    assert _need(t, k, n, group)[0] > 0
+    parts = _weight(n, k, group, True, dtype, seed=70)
+    x, bias = _x(t, k, dtype, seed=71), _x(1, n, dtype, seed=72)[0]
+    w, s = codes64(*parts)
+    want, bound = dot_bound(x, w, s, group)
+    packed = w4.pack_w4(*_dev(parts))
+    got = [w4.linear_w4(x.to(DEV), packed) for _ in range(4)]
+    check(got[0], want, bound)
+    assert all(torch.equal(g, got[0]) for g in got)
+    biased = w4.linear_w4(x.to(DEV), packed, bias.to(DEV))
+    y = want + bias.double()
+    check(biased, y, bound + 2.0 ** -23 * y.abs())
+
+
+def test_split_shapes_take_turns_graphs_and_threads():
+    """Calls of several shapes on one workspace; two graphs at once beside eager calls; two host threads."""
+    shapes = [(24, 1024, 8192), (61, 200, 12288), (17, 48, 16384), (3, 64, 4096), (24, 1024, 8192)]
+    packs = [w4.pack_w4(*_dev(_weight(n, k, 128, False, BF, seed=80 + i))) for i, (_, n, k) in enumerate(shapes)]
+    xs = [_x(t, k, BF, seed=90 + i).to(DEV) for i, (t, _, k) in enumerate(shapes)]
+    assert sum(_need(t, k, n, 128)[0] > 0 for t, n, k in shapes) >= 4
+    want = [w4.linear_w4(x, p) for x, p in zip(xs, packs)]
+    for _ in range(3):
+        for x, p, y in zip(xs, packs, want):
+            assert torch.equal(w4.linear_w4(x, p), y)
+    one, graphs, outs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=one):
+            outs.append([w4.linear_w4(x, p) for x, p in zip(xs, packs)])
+        graphs.append(g)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for g, s in zip(graphs, sides):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(one):
+            eager = [w4.linear_w4(x, p) for x, p in zip(xs, packs)]
+        torch.cuda.synchronize()
+        for got in (*outs, eager):
+            assert all(torch.equal(o, y) for o, y in zip(got, want))
+    got = [[], []]
+    threads = [threading.Thread(target=lambda i=i: got[i].extend(w4.linear_w4(xs[i], packs[i]) for _ in range(50)))
+               for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(len(g) == 50 and all(torch.equal(o, want[i]) for o in g) for i, g in enumerate(got))
+
+
+def test_split_with_and_without_a_workspace(monkeypatch):
+    lib = _lib.load()
+    t, n, k, group = 24, 1024, 8192, 128
+    parts = _weight(n, k, group, False, BF, seed=100)
+    packed, x = w4.pack_w4(*_dev(parts)), _x(t, k, BF, seed=101).to(DEV)
+    need, counters = _need(t, k, n, group)
+    ws, out = torch.zeros(need, dtype=torch.uint8, device=DEV), torch.empty(t, n, dtype=BF, device=DEV)
+
+    def call(space, size):
+        return lib.ember_w4_linear_split(x.data_ptr(), k, packed.packed.data_ptr(), group, 2, t, k, n, None, space, size,
+                                         out.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+
+    assert call(ws.data_ptr(), need - 16) == 1 and call(ws.data_ptr(), need - 8) == 2  # before any launch
+    assert call(ws.data_ptr() + 8, need) == 2
+    want, bound = dot_bound(x.cpu(), *codes64(*parts), group)
+    for space, size in ((ws.data_ptr(), need), (None, 0)):
+        out.zero_()
+        assert call(space, size) == 0
+        check(out, want, bound)
+    assert not bool(ws[need - counters:].any())
+    eager = w4.linear_w4(x, packed)
+    monkeypatch.setenv("EMBERSERVE_CHECK_INDICES", "1")  # the wrapper's path, which looks at the counters
+    assert torch.equal(w4.linear_w4(x, packed), eager)
+
+
 def test_rows_far_apart_are_copied():
     """Row strides past what 32-bit offsets reach over 64 rows."""
     parts = _weight(48, 128, 64, False, BF, seed=52)
@@ -218,7 +307,6 @@ def test_more_threads_than_one_launch_takes():
 
 def test_two_threads_on_one_stream():
     """Calls of two host threads, each into its own output."""
-    import threading
     parts = _weight(256, 1024, 128, False, BF, seed=56)
     packed = w4.pack_w4(*_dev(parts))
     xs = [_x(5 + 8 * i, 1024, BF, seed=57 + i).to(DEV) for i in range(2)]

@@ -232,6 +232,23 @@ def test_abi_argument_checks():
     assert down(p, 0, 64, 2, 0, 16, 64, p, None) == 1 and down(p, 0, 64, 2, 1, 20, 64, p, None) == 1
 
 
+def test_abi_checks_of_the_split_form():
+    lib = _lib.load()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4100)
+    cnt = ctypes.c_int64(7)
+    size = lib.ember_w4_linear_workspace_bytes
+    assert size(1, 4096, 4096, 128, ctypes.byref(cnt)) == 0 and cnt.value == 0  # one token: no splits
+    assert size(1 << 20, 4096, 4096, 128, None) == 0
+    for bad in ((-1, 128, 16, 128), (1, 128, 0, 128), (1, 100, 16, 32), (1, 128, 16, 96), (1 << 22, 128, 16, 128)):
+        assert size(*bad, None) == -1
+    lin = lib.ember_w4_linear_split
+    assert lin(p, 128, p, 128, 2, 0, 128, 16, None, None, 0, p, 16, None) == 0
+    assert lin(p, 128, p, 128, 2, 1, 128, 16, None, odd, 256, p, 16, None) == 2
+    assert lin(p, 128, p, 128, 2, 1, 128, 16, None, p, 250, p, 16, None) == 2
+    assert lin(None, 128, p, 128, 2, 1, 128, 16, None, p, 256, p, 16, None) == 1
+    assert lin(p, (1 << 23) + 8, p, 128, 2, 1, 128, 16, None, p, 256, p, 16, None) == 1
+
+
 def test_bounds_have_teeth():
     """The oracle's bound refuses a wrong zero point, scale or expert."""
     q, s, z = w4.quantize_w4(_w(16, 256), 64, symmetric=False)
