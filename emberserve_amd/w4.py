@@ -47,6 +47,8 @@ def quantize_w4(weight: Tensor, group_size: int = 128, *, symmetric: bool = True
                          f"{weight.dtype}")
     k = weight.shape[-1]
     _check_group(k, group_size)
+    if not bool(torch.isfinite(weight).all()):
+        raise ValueError("quantize_w4: the weight has infinities or NaN")
     w = weight.float().reshape(*weight.shape[:-1], k // group_size, group_size)
     # a group of zeros: any scale, codes at the zero point. fp16 weights under 2^-11 have scales below
     # its normal range, whose smallest step is 2^-24

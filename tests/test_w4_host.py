@@ -38,6 +38,14 @@ def test_quantize_rounds_to_nearest(dtype, symmetric, group):
     assert bool((d[3, :group] == 0).all())
 
 
+def test_quantize_refuses_what_is_not_finite():
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        w = _w(4, 64)
+        w[2, 5] = bad
+        with pytest.raises(ValueError):
+            w4.quantize_w4(w, 32)
+
+
 @pytest.mark.parametrize("symmetric", [True, False])
 def test_quantize_small_fp16_weights(symmetric):
     """Scales below fp16's normal range are multiples of 2^-24: half of one more a code for the scale's
